@@ -12,7 +12,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm355dist.so")
 
-F64, F32, I64 = 0, 1, 2
+F64, F32, I64, F16, BF16, I32 = 0, 1, 2, 3, 4, 5
 # distribution ids of include/m355_dist.h (enum m355_dist) and the reference's parameter names, in order
 PARAMS = {
     "normal": ('mu', 'sigma'),
@@ -79,6 +79,42 @@ class Operand(ctypes.Structure):
         ("scalar", ctypes.c_double),
         ("div", ctypes.c_int64),
         ("mod", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class LogitAdjust(ctypes.Structure):
+    """m355_logit_adjust of include/m355_dist.h."""
+
+    _fields_ = [
+        ("history", ctypes.c_void_p),
+        ("history_len", ctypes.c_int64),
+        ("history_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("prompt_lengths", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("bias_stride", ctypes.c_int64),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("history_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("mask_kind", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("repetition", Operand),
+        ("presence", Operand),
+        ("frequency", Operand),
+        ("temperature", Operand),
+    ]
+
+
+class Tensor(ctypes.Structure):
+    """m355_tensor of include/m355_dist.h."""
+
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
         ("dtype", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
     ]

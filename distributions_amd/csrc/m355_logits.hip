@@ -1,0 +1,608 @@
+// Categorical given by logits: adjustment before drawing or scoring (penalties, bias, temperature, mask) with its
+// gradient, log-density and the gradient of the weighted sum of log-densities.  Formulas: include/m355_dist.h.
+#include <hip/hip_runtime.h>
+
+#include "m355_error.h"
+#include "m355_logits_io.h"
+
+namespace m355 {
+
+// ------------------------------------------------------------------------------------------------ adjust
+struct AdjustArgs {
+  long long rows, k;
+  const void* src;  // the logits (forward) or g (gradient)
+  long long src_ld;
+  const void* x;  // gradient: the logits, for the sign of the penalised ones
+  long long x_ld;
+  void* dst;  // NULL: not wanted (gradient)
+  long long dst_ld;
+  void* dbias;  // gradient: per-element gradient of the bias (rows x k), or NULL
+  const void* history;
+  long long history_ld;
+  int history_len, history_dtype;
+  const long long *lengths, *prompts;
+  DevOperand rep, pres, freq, temp;
+  const void* bias;
+  long long bias_ld;
+  int bias_dtype;
+  int mask_kind;
+  const void* mask;
+  long long mask_ld;
+};
+
+// kPer flags for the elements from v on (v is a multiple of kPer): bit e = element v + e is allowed
+template <class T> M355_DEV unsigned mask_flags(const AdjustArgs& a, long long row, long long v) {
+  constexpr int N = kPer<T>;
+  if (a.mask_kind == M355_MASK_NONE) return (1u << N) - 1;
+  if (a.mask_kind == M355_MASK_BITS) {
+    const unsigned w = static_cast<const unsigned*>(a.mask)[row * a.mask_ld + (v >> 5)];
+    return (w >> (v & 31)) & ((1u << N) - 1);
+  }
+  const unsigned char* m = static_cast<const unsigned char*>(a.mask) + row * a.mask_ld + v;
+  unsigned f = 0;
+  if (v + N <= a.k) {
+    unsigned char b[N];
+    __builtin_memcpy(b, m, N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f |= (b[e] != 0 ? 1u : 0u) << e;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (v + e < a.k) f |= (m[e] != 0 ? 1u : 0u) << e;
+  }
+  return f;
+}
+
+template <class T> M355_DEV void load_bias(const AdjustArgs& a, long long row, long long v, typename T::comp (&b)[kPer<T>]) {
+  if (a.bias_dtype == T::kCode) {
+    unpack<T>(load_row<T>(static_cast<const typename T::store*>(a.bias) + row * a.bias_ld, v, a.k, 0), b);
+  } else {  // float32 next to 16-bit logits
+    const float* p = static_cast<const float*>(a.bias) + row * a.bias_ld;
+#pragma unroll
+    for (int h = 0; h < kPer<T>; h += 4) {
+      float t[4];
+      unpack<F32>(load_row<F32>(p, v + h < a.k ? v + h : 0, v + h < a.k ? a.k : 0, 0.0f), t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (h + e < kPer<T>) b[h + e] = (typename T::comp)t[e];
+    }
+  }
+}
+
+constexpr int kAdjThreads = 256;
+
+// One workgroup per (row, chunk of kAdjThreads * VPT * kPer categories).  With a history the workgroup first counts the
+// ids that fall into its chunk in LDS (word = 2 * generated + [in the prompt]: one atomic per id), then streams its chunk.
+template <class T, int VPT, bool HIST, bool BWD>
+__global__ __launch_bounds__(kAdjThreads) void k_logits_adjust(const AdjustArgs a, long long items, int chunks) {
+  constexpr int N = kPer<T>;
+  constexpr int C = kAdjThreads * VPT * N;
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  extern __shared__ unsigned counts[];  // C words with HIST
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long long row = item / chunks;
+    const long long base = (item - row * chunks) * C;
+    const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
+    raw_t<T> raw[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const long long v = base + (j * kAdjThreads + threadIdx.x) * N;
+      if (v < a.k) raw[j] = load_row<T>(src, v, a.k, 0);
+    }
+    comp rep = 1, pres = 0, freq = 0;
+    if constexpr (HIST) {
+#pragma unroll
+      for (int j = 0; j < VPT * N / 4; ++j)
+        reinterpret_cast<uint4*>(counts)[j * kAdjThreads + threadIdx.x] = uint4{0, 0, 0, 0};
+      __syncthreads();
+      const long long left = a.k - base;
+      const unsigned long long width = left < C ? left : C;
+      long long len = a.lengths ? a.lengths[row] : a.history_len;
+      len = len < 0 ? 0 : (len > a.history_len ? a.history_len : len);
+      const long long prompt = a.prompts ? a.prompts[row] : 0;
+      for (int i = threadIdx.x; i < (int)len; i += kAdjThreads) {
+        const long long id = a.history_dtype == M355_I64
+                                 ? static_cast<const long long*>(a.history)[row * a.history_ld + i]
+                                 : (long long)static_cast<const int*>(a.history)[row * a.history_ld + i];
+        const unsigned long long at = (unsigned long long)(id - base);
+        if (id >= 0 && at < width) {
+          if (i >= prompt) atomicAdd(&counts[at], 2u);
+          else atomicOr(&counts[at], 1u);
+        }
+      }
+      __syncthreads();
+      rep = (comp)row_operand(a.rep, row);
+      pres = (comp)row_operand(a.pres, row);
+      freq = (comp)row_operand(a.freq, row);
+    }
+    // one rounding more than a division per element, which would cost more than the rest of the body
+    const comp inv_t = (comp)(1.0 / row_operand(a.temp, row));
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int at = (j * kAdjThreads + threadIdx.x) * N;
+      const long long v = base + at;
+      if (v >= a.k) continue;
+      comp s[N];
+      unpack<T>(raw[j], s);
+      const unsigned ok = mask_flags<T>(a, row, v);
+      if constexpr (!BWD) {
+        if constexpr (HIST) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const unsigned c = counts[at + e];
+            if (c) {
+              s[e] = s[e] > 0 ? s[e] / rep : s[e] * rep;
+              if (c >> 1) s[e] -= freq * (comp)(c >> 1) + pres;
+            }
+          }
+        }
+        if (a.bias) {
+          comp b[N];
+          load_bias<T>(a, row, v, b);
+#pragma unroll
+          for (int e = 0; e < N; ++e) s[e] += b[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)-kInf;
+        store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)0;
+        if (a.dbias) {
+          if (a.bias_dtype == T::kCode) {
+            store_row<T>(static_cast<store*>(a.dbias) + row * a.k, v, a.k, s);
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (v + e < a.k) static_cast<float*>(a.dbias)[row * a.k + v + e] = (float)s[e];
+          }
+        }
+        if (!a.dst) continue;
+        if constexpr (HIST) {
+          const store* x = static_cast<const store*>(a.x) + row * a.x_ld;
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (counts[at + e]) s[e] = (comp)x[v + e] > 0 ? s[e] / rep : s[e] * rep;
+        }
+        store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+      }
+    }
+    if constexpr (HIST) __syncthreads();  // the next item clears the counts
+  }
+}
+
+// Gradient of a bias that all rows share: a thread owns kPer columns and walks a block of rows, so that the column sums
+// stay in its registers (float64); the partial sums of the row blocks are added in order by k_logits_cols_final.
+// Without a history the gradient of the logits is written on the way.
+template <class T, bool WRITE>
+__global__ __launch_bounds__(kAdjThreads) void k_logits_adjust_cols(const AdjustArgs a, int chunks, int row_blocks,
+                                                                    double* __restrict__ partials) {
+  constexpr int N = kPer<T>;
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  const int chunk = blockIdx.x % chunks, rb = blockIdx.x / chunks;
+  const long long v = ((long long)chunk * kAdjThreads + threadIdx.x) * N;
+  if (v >= a.k) return;
+  const long long lo = a.rows * rb / row_blocks, hi = a.rows * (rb + 1) / row_blocks;
+  double acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.0;
+  for (long long row = lo; row < hi; ++row) {
+    comp s[N];
+    unpack<T>(load_row<T>(static_cast<const store*>(a.src) + row * a.src_ld, v, a.k, 0), s);
+    const unsigned ok = mask_flags<T>(a, row, v);
+    const comp inv_t = (comp)(1.0 / row_operand(a.temp, row));
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)0;
+      acc[e] += (double)s[e];
+    }
+    if constexpr (WRITE) store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (v + e < a.k) partials[(long long)rb * a.k + v + e] = acc[e];
+}
+
+template <class T>
+__global__ __launch_bounds__(kAdjThreads) void k_logits_cols_final(const double* __restrict__ partials, long long k,
+                                                                   int row_blocks, void* __restrict__ out, int odt) {
+  const long long v = (long long)blockIdx.x * kAdjThreads + threadIdx.x;
+  if (v >= k) return;
+  double s = 0.0;
+  for (int b = 0; b < row_blocks; ++b) s += partials[(long long)b * k + v];
+  if (odt == T::kCode) static_cast<typename T::store*>(out)[v] = (typename T::store)s;
+  else static_cast<float*>(out)[v] = (float)s;
+}
+
+// ----------------------------------------------------------------------------------------- log-density
+// exp(d) for d <= 0 (d > 0 only where the row holds +inf): 2^(d log2 e) with the product's rounding error carried along,
+// relative error below 2^-22 wherever the result is a normal float, 0 below; NaN stays NaN.
+M355_DEV float exp_neg(float d) {
+  const float t = d * 1.44269502f;                              // float(log2 e)
+  const float r = __builtin_fmaf(d, 1.44269502f, -t) + d * 1.92596303e-8f;  // log2 e - float(log2 e)
+  const float p = __builtin_amdgcn_exp2f(t);
+  return d < -87.0f ? 0.0f : __builtin_fmaf(p, r * 0.693147182f, p);
+}
+M355_DEV double exp_neg(double d) { return ::exp(d); }
+M355_DEV float log_c(float v) { return ::logf(v); }
+M355_DEV double log_c(double v) { return ::log(v); }
+
+struct DensityArgs {
+  long long rows, k;
+  const void* z;
+  long long z_ld;
+  const void* x;
+  int x_dtype;
+  void* lp;  // rows values of the arithmetic type
+  DevOperand weight;
+  void* grad;  // NULL: value only
+  long long grad_ld;
+};
+
+// The observation of a row as a category, or -1
+M355_DEV long long observed(const DensityArgs& a, long long row) {
+  if (a.x_dtype == M355_I64 || a.x_dtype == M355_I32) {
+    const long long i = a.x_dtype == M355_I64 ? static_cast<const long long*>(a.x)[row]
+                                              : (long long)static_cast<const int*>(a.x)[row];
+    return i >= 0 && i < a.k ? i : -1;
+  }
+  const double v = load1(a.x, a.x_dtype, (unsigned long long)row);
+  return v >= 0.0 && v < (double)a.k && v == floor_(v) ? (long long)v : -1;
+}
+
+M355_DEV float max_c(float a, float b) { return __builtin_fmaxf(a, b); }  // a NaN is left out: the sum holds it
+M355_DEV double max_c(double a, double b) { return __builtin_fmax(a, b); }
+template <class C> M355_DEV C finite_max(C m) { return m == (C)-kInf ? (C)0 : m; }
+
+// (m, s) of two parts of a row: the running maximum and the sum of exp(z - m), with m taken as 0 where a part is all -inf
+template <class C> M355_DEV void join(C& m, C& s, C m2, C s2) {
+  const C mm = max_c(m, m2);
+  const C b = finite_max(mm);
+  s = s * exp_neg(m - b) + s2 * exp_neg(m2 - b);
+  m = mm;
+}
+
+template <class T> M355_DEV void accumulate(const typename T::comp (&z)[kPer<T>], typename T::comp& m, typename T::comp& s) {
+  typedef typename T::comp comp;
+  comp mv = z[0];
+#pragma unroll
+  for (int e = 1; e < kPer<T>; ++e) mv = max_c(mv, z[e]);
+  if (mv > m) {
+    s *= exp_neg(m - mv);  // m = -inf: 0
+    m = mv;
+  }
+  const comp b = finite_max(m);
+#pragma unroll
+  for (int e = 0; e < kPer<T>; ++e) s += exp_neg(z[e] - b);
+}
+
+template <int THREADS, class C> M355_DEV void block_join(C& m, C& s) {
+  __shared__ C red[2][THREADS / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) join<C>(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) {
+    red[0][wave] = m;
+    red[1][wave] = s;
+  }
+  __syncthreads();
+  m = red[0][0];
+  s = red[1][0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) join<C>(m, s, red[0][w], red[1][w]);
+  __syncthreads();
+}
+
+// log-density from the row's statistics; -inf for an observation that is no category and for a row that is all -inf
+template <class C> M355_DEV C density(C zx, C m, C s, bool inside) {
+  return !inside || s == (C)0 ? (C)-kInf : (zx - finite_max(m)) - log_c(s);
+}
+
+// One workgroup per row: one pass for the running maximum and sum, one more over the row for the gradient.
+template <class T, int THREADS, bool GRAD>
+__global__ __launch_bounds__(THREADS) void k_logits_density(const DensityArgs a) {
+  constexpr int N = kPer<T>;
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const store* z = static_cast<const store*>(a.z) + row * a.z_ld;
+    const comp w = GRAD ? (comp)row_operand(a.weight, row) : (comp)1;
+    const long long xi = observed(a, row);
+    const comp zx = xi >= 0 ? (comp)z[xi] : (comp)0;
+    comp m = (comp)-kInf, s = 0;
+    if (!GRAD || w != (comp)0) {
+      for (long long v = (long long)threadIdx.x * N; v < a.k; v += THREADS * N) {
+        comp t[N];
+        unpack<T>(load_row<T>(z, v, a.k, (comp)-kInf), t);
+        accumulate<T>(t, m, s);
+      }
+      block_join<THREADS>(m, s);  // its barriers also separate the read of z[xi] from the writes of the gradient
+    }
+    if (threadIdx.x == 0) static_cast<comp*>(a.lp)[row] = density(zx, m, s, xi >= 0);
+    if constexpr (GRAD) {
+      store* g = static_cast<store*>(a.grad) + row * a.grad_ld;
+      const comp b = finite_max(m);
+      const bool zero = w == (comp)0 || xi < 0 || s == (comp)0;
+      const comp q = zero ? (comp)0 : -w / s;
+      for (long long v = (long long)threadIdx.x * N; v < a.k; v += THREADS * N) {
+        comp t[N];
+        if (zero) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) t[e] = 0;
+        } else {
+          unpack<T>(load_row<T>(z, v, a.k, (comp)-kInf), t);
+#pragma unroll
+          for (int e = 0; e < N; ++e) t[e] = exp_neg(t[e] - b) * q + (v + e == xi ? w : (comp)0);
+        }
+        store_row<T>(g, v, a.k, t);
+      }
+    }
+  }
+}
+
+// total = sum over rows of w * lp in a fixed order; a row of weight 0 is left out whatever its density
+template <class C>
+__global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp, DevOperand weight, long long rows,
+                                                       C* __restrict__ total) {
+  __shared__ double red[16];
+  double acc = 0.0;
+  for (long long r = threadIdx.x; r < rows; r += 1024) {
+    const double w = row_operand(weight, r);
+    if (w != 0.0) acc += w * (double)lp[r];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) acc += __shfl_down(acc, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) acc += red[i];
+    total[0] = (C)acc;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- launches
+constexpr long long kMaxGrid = 1ll << 30;
+
+template <class T, int VPT, bool HIST, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+  constexpr int C = kAdjThreads * VPT * kPer<T>;
+  const long long chunks = (a.k + C - 1) / C, items = a.rows * chunks;
+  hipLaunchKernelGGL((k_logits_adjust<T, VPT, HIST, BWD>), dim3((unsigned)(items < kMaxGrid ? items : kMaxGrid)),
+                     dim3(kAdjThreads), HIST ? C * sizeof(unsigned) : 0, s, a, items, (int)chunks);
+}
+
+template <class T, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+  if (a.history) launch_adjust<T, 4, true, BWD>(a, s);
+  else launch_adjust<T, 4, false, BWD>(a, s);
+}
+
+// row blocks of k_logits_adjust_cols: enough workgroups to fill the chip, at least eight rows each
+template <class T> int row_blocks_of(long long rows, long long k) {
+  const long long chunks = (k + kAdjThreads * kPer<T> - 1) / (kAdjThreads * kPer<T>);
+  long long rb = 2048 / chunks;
+  if (rb > rows / 8) rb = rows / 8;
+  return (int)(rb < 1 ? 1 : rb);
+}
+
+template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, double* ws, hipStream_t s) {
+  const int chunks = (int)((a.k + kAdjThreads * kPer<T> - 1) / (kAdjThreads * kPer<T>));
+  const int rb = row_blocks_of<T>(a.rows, a.k);
+  const dim3 grid((unsigned)((long long)chunks * rb)), block(kAdjThreads);
+  if (a.dst) hipLaunchKernelGGL((k_logits_adjust_cols<T, true>), grid, block, 0, s, a, chunks, rb, ws);
+  else hipLaunchKernelGGL((k_logits_adjust_cols<T, false>), grid, block, 0, s, a, chunks, rb, ws);
+  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + kAdjThreads - 1) / kAdjThreads)), block, 0, s, ws,
+                     a.k, rb, dbias, a.bias_dtype);
+}
+
+template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid);
+  hipLaunchKernelGGL((k_logits_density<T, 256, GRAD>), dim3(grid), dim3(256), 0, s, a);
+}
+
+template <class F> int by_dtype(int dtype, F f) {
+  switch (dtype) {
+    case M355_F64: return f(F64());
+    case M355_F32: return f(F32());
+    case M355_F16: return f(F16());
+    case M355_BF16: return f(BF16());
+  }
+  return fail(M355_ERR_INVALID, "logits are float64, float32, float16 or bfloat16 (dtype %d)", dtype);
+}
+
+}  // namespace m355
+
+namespace {
+using m355::fail;
+
+int launched() {
+  hipError_t e = hipGetLastError();
+  return e == hipSuccess ? M355_OK : fail(M355_ERR_LAUNCH, "HIP launch failed: %s", hipGetErrorString(e));
+}
+
+int check_rows(int64_t rows, int64_t k, int dtype) {
+  if (rows < 0) return fail(M355_ERR_INVALID, "rows must be >= 0");
+  if (k < 1 || k > INT32_MAX) return fail(M355_ERR_INVALID, "1 <= k < 2^31 categories, got %lld", (long long)k);
+  return m355::by_dtype(dtype, [](auto) { return 0; });
+}
+
+int row_arg(const m355_operand& in, int64_t rows, m355::DevOperand& out, const char* what) {
+  out.ptr = in.ptr;
+  out.scalar = in.scalar;
+  out.dtype = in.dtype;
+  out.div = 1;
+  out.mod = 1;
+  if (!in.ptr) return 0;
+  if (in.dtype != M355_F64 && in.dtype != M355_F32) return fail(M355_ERR_INVALID, "%s: float64 or float32", what);
+  if (in.div < 1 || in.mod < 1) return fail(M355_ERR_INVALID, "%s: div and mod must be >= 1", what);
+  out.div = (unsigned long long)in.div;
+  out.mod = in.div >= rows ? 1 : (unsigned long long)in.mod;
+  return 0;
+}
+
+int check_adjust(int64_t rows, int64_t k, int dtype, const m355_logit_adjust* d, m355::AdjustArgs& a) {
+  if (!d) return fail(M355_ERR_INVALID, "NULL adjustment");
+  a = m355::AdjustArgs();
+  a.rows = rows;
+  a.k = k;
+  if (d->history_len < 0 || d->history_len > INT32_MAX || d->history_stride < 0)
+    return fail(M355_ERR_INVALID, "0 <= history_len < 2^31, history_stride >= 0");
+  if (d->history && d->history_len) {
+    if (d->history_dtype != M355_I64 && d->history_dtype != M355_I32)
+      return fail(M355_ERR_INVALID, "history ids are int64 or int32");
+    a.history = d->history;
+  }
+  a.history_ld = d->history_stride;
+  a.history_len = (int)d->history_len;
+  a.history_dtype = d->history_dtype;
+  a.lengths = reinterpret_cast<const long long*>(d->lengths);
+  a.prompts = reinterpret_cast<const long long*>(d->prompt_lengths);
+  if (d->bias && d->bias_dtype != dtype && !(d->bias_dtype == M355_F32 && (dtype == M355_F16 || dtype == M355_BF16)))
+    return fail(M355_ERR_INVALID, "the bias has the dtype of the logits, or float32 with 16-bit logits");
+  if (d->bias_stride < 0 || d->mask_stride < 0) return fail(M355_ERR_INVALID, "negative stride");
+  a.bias = d->bias;
+  a.bias_ld = d->bias_stride;
+  a.bias_dtype = d->bias_dtype;
+  if (d->mask_kind < M355_MASK_NONE || d->mask_kind > M355_MASK_BITS || (d->mask_kind && !d->mask))
+    return fail(M355_ERR_INVALID, "bad mask");
+  a.mask_kind = d->mask_kind;
+  a.mask = d->mask;
+  a.mask_ld = d->mask_stride;
+  int rc;
+  if ((rc = row_arg(d->repetition, rows, a.rep, "repetition")) || (rc = row_arg(d->presence, rows, a.pres, "presence")) ||
+      (rc = row_arg(d->frequency, rows, a.freq, "frequency")) ||
+      (rc = row_arg(d->temperature, rows, a.temp, "temperature")))
+    return rc;
+  return 0;
+}
+
+int check_density(int64_t rows, int64_t k, int dtype, const void* logits, int64_t stride, const void* x, int x_dtype,
+                  m355::DensityArgs& a) {
+  const int rc = check_rows(rows, k, dtype);
+  if (rc) return rc;
+  if (x_dtype != M355_I64 && x_dtype != M355_I32 && x_dtype != M355_F64 && x_dtype != M355_F32)
+    return fail(M355_ERR_INVALID, "observations are int64, int32, float64 or float32");
+  if (stride < 0) return fail(M355_ERR_INVALID, "negative stride");
+  if (rows && (!logits || !x)) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  a = m355::DensityArgs();
+  a.rows = rows;
+  a.k = k;
+  a.z = logits;
+  a.z_ld = stride;
+  a.x = x;
+  a.x_dtype = x_dtype;
+  return 0;
+}
+}  // namespace
+
+extern "C" int m355_logits_adjust(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
+                                  const m355_logit_adjust* adjust, void* out, int64_t out_stride, void* stream) {
+  using namespace m355;
+  AdjustArgs a;
+  int rc = check_rows(rows, k, dtype);
+  if (!rc) rc = check_adjust(rows, k, dtype, adjust, a);
+  if (rc) return rc;
+  if (logits_stride < 0 || (rows > 1 && out_stride < k)) return fail(M355_ERR_INVALID, "bad row stride");
+  if (rows == 0) return M355_OK;
+  if (!logits || !out) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  a.src = logits;
+  a.src_ld = logits_stride;
+  a.dst = out;
+  a.dst_ld = out_stride;
+  by_dtype(dtype, [&](auto t) { return launch_adjust<decltype(t), false>(a, static_cast<hipStream_t>(stream)), 0; });
+  return launched();
+}
+
+extern "C" size_t m355_logits_adjust_grad_workspace_bytes(int64_t rows, int64_t k, int dtype) {
+  if (rows < 1 || k < 1 || k > INT32_MAX) return 0;
+  int rb = 0;
+  m355::by_dtype(dtype, [&](auto t) { return (rb = m355::row_blocks_of<decltype(t)>(rows, k)), 0; });
+  return (size_t)rb * (size_t)k * sizeof(double);
+}
+
+extern "C" int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const void* g, int64_t g_stride,
+                                       const void* logits, int64_t logits_stride, const m355_logit_adjust* adjust,
+                                       void* dlogits, void* dbias, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  using namespace m355;
+  AdjustArgs a;
+  int rc = check_rows(rows, k, dtype);
+  if (!rc) rc = check_adjust(rows, k, dtype, adjust, a);
+  if (rc) return rc;
+  if (g_stride < 0 || logits_stride < 0) return fail(M355_ERR_INVALID, "bad row stride");
+  if (dbias && !a.bias) return fail(M355_ERR_INVALID, "dbias without a bias");
+  const bool shared = dbias && a.bias_ld == 0;
+  if (rows == 0 && !shared) return M355_OK;
+  if ((rows && (!g || (dlogits && a.history && !logits)))) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (shared && rows && (!workspace || workspace_bytes < m355_logits_adjust_grad_workspace_bytes(rows, k, dtype)))
+    return fail(M355_ERR_WORKSPACE, "workspace too small");
+  a.src = g;
+  a.src_ld = g_stride;
+  a.x = logits;
+  a.x_ld = logits_stride;
+  a.dst = dlogits;
+  a.dst_ld = k;
+  a.dbias = shared ? nullptr : dbias;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  by_dtype(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (shared) {
+      AdjustArgs c = a;
+      if (a.history) c.dst = nullptr;  // the row kernel writes the gradient of the logits
+      launch_adjust_cols<T>(c, dbias, static_cast<double*>(workspace), s);
+    }
+    if ((a.dst && (!shared || a.history)) || a.dbias) launch_adjust<T, true>(a, s);
+    return 0;
+  });
+  return launched();
+}
+
+extern "C" size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype) {
+  (void)k;
+  (void)dtype;
+  return (size_t)(rows > 0 ? rows : 0) * sizeof(double);
+}
+
+extern "C" int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
+                                  const void* x, int x_dtype, void* out, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  using namespace m355;
+  DensityArgs a;
+  const int rc = check_density(rows, k, dtype, logits, logits_stride, x, x_dtype, a);
+  if (rc) return rc;
+  if (rows == 0) return M355_OK;
+  if (!out || !workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (workspace_bytes < m355_logits_workspace_bytes(rows, k, dtype)) return fail(M355_ERR_WORKSPACE, "workspace too small");
+  a.lp = out;
+  by_dtype(dtype, [&](auto t) { return launch_density<decltype(t), false>(a, static_cast<hipStream_t>(stream)), 0; });
+  return launched();
+}
+
+extern "C" int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
+                                           const void* x, int x_dtype, const m355_operand* weights, void* total,
+                                           void* dlogits, int64_t dlogits_stride, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  using namespace m355;
+  DensityArgs a;
+  int rc = check_density(rows, k, dtype, logits, logits_stride, x, x_dtype, a);
+  if (rc) return rc;
+  if (!weights || !total) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if ((rc = row_arg(*weights, rows, a.weight, "weights"))) return rc;
+  if (dlogits && rows > 1 && dlogits_stride < k) return fail(M355_ERR_INVALID, "bad row stride");
+  if (rows && !workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (workspace_bytes < m355_logits_workspace_bytes(rows, k, dtype)) return fail(M355_ERR_WORKSPACE, "workspace too small");
+  a.lp = workspace;
+  a.grad = dlogits;
+  a.grad_ld = dlogits_stride;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  by_dtype(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    typedef typename T::comp comp;
+    if (rows && dlogits) launch_density<T, true>(a, s);
+    else if (rows) launch_density<T, false>(a, s);
+    hipLaunchKernelGGL((k_logits_total<comp>), dim3(1), dim3(1024), 0, s, static_cast<const comp*>(a.lp), a.weight,
+                       (long long)rows, static_cast<comp*>(total));
+    return 0;
+  });
+  return launched();
+}

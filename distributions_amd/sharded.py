@@ -57,3 +57,14 @@ def total_loglik(terms: Sequence[tuple], group=None):
         raw.sumlogp_into(name, "logpdf", x, params, sums[i:], ws)
     allreduce_sum_(sums, group)
     return sums, sums.sum()
+
+
+def clip_global_norm(grads, max_norm, out=None, group=None):
+    """gradients.clip_global_norm over the gradients of all ranks: each rank passes its own shards (disjoint parts of the
+    whole; a gradient that every rank holds would count once per rank), the sums of squares are added by one all-reduce of
+    8 bytes, and each rank scales its shards by the common factor.  Returns (norm over all ranks, clipped shards)."""
+    from . import _gradnorm
+
+    sumsq = _gradnorm.global_norm(grads, sumsq_only=True)
+    allreduce_sum_(sumsq, group)
+    return _gradnorm.clip_global_norm(grads, max_norm, out, sumsq)

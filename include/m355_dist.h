@@ -42,7 +42,8 @@ enum m355_status {
   M355_ERR_WORKSPACE = -4    /* workspace too small */
 };
 
-enum m355_dtype { M355_F64 = 0, M355_F32 = 1, M355_I64 = 2 };
+/* F16 / BF16: logits and lists of gradients only; I32: observations of the logits calls and token histories only */
+enum m355_dtype { M355_F64 = 0, M355_F32 = 1, M355_I64 = 2, M355_F16 = 3, M355_BF16 = 4, M355_I32 = 5 };
 
 /* distribution ids: the reference module each one replaces */
 enum m355_dist {
@@ -346,6 +347,99 @@ int m355_multinomial_logpdf(int64_t rows, int k, const void* x, int x_dtype, con
  * row, rows x k int64 out; row r uses Philox counter counter_offset + r. */
 int m355_multinomial_rvs(int64_t rows, int k, double n, const double* p, uint64_t seed, uint32_t stream_id,
                          uint64_t counter_offset, int64_t* out, void* stream);
+
+/*
+ * Categorical given by logits, one row z of k unnormalised log-weights per observation (no counterpart in the reference,
+ * whose categorical takes one probability vector).  `dtype` is M355_F64 / F32 / F16 / BF16; rows are `*_stride` elements
+ * apart (64-bit offsets), their elements are contiguous, any element alignment is accepted.  Arithmetic is float64 for
+ * F64 and float32 otherwise; the value outputs (log-density, total) are float64 resp. float32.
+ *
+ * m355_logits_adjust: what is done to logits before they are drawn from or scored,
+ *     s = z[v];  c_all > 0: s = s > 0 ? s / repetition : s * repetition;
+ *     s -= frequency * c_gen + presence * (c_gen > 0);  s += bias[v];  s /= temperature;  v not allowed: s = -inf
+ * with c_all[v] the number of i < lengths[r] and c_gen[v] of prompt_lengths[r] <= i < lengths[r] with history[r, i] == v;
+ * ids outside [0, k) are skipped, lengths are clamped to [0, history_len].  out (rows x k of dtype) may be the logits
+ * themselves (same address and stride); any other overlap with an input is undefined.
+ * repetition / presence / frequency / temperature: operands as in m355_elemwise over the row index, float64 or float32
+ * arrays (repetition and temperature are positive; other values follow the formula).
+ */
+enum m355_mask_kind {
+  M355_MASK_NONE = 0,
+  M355_MASK_BYTES = 1, /* one byte per category, 0 = not allowed */
+  M355_MASK_BITS = 2   /* category v is bit v % 32 of the 32-bit word v / 32; 1 = allowed */
+};
+typedef struct m355_logit_adjust {
+  const void* history;           /* rows x history_len ids, or NULL: no penalties */
+  int64_t history_len;           /* < 2^31 */
+  int64_t history_stride;        /* elements between rows, 0: one history shared by all rows */
+  const int64_t* lengths;        /* rows entries, or NULL: history_len */
+  const int64_t* prompt_lengths; /* rows entries, or NULL: 0 */
+  const void* bias;              /* k or rows x k values, or NULL */
+  int64_t bias_stride;           /* elements between rows, 0: shared by all rows */
+  const void* mask;              /* k or rows x k flags, or NULL with M355_MASK_NONE */
+  int64_t mask_stride;           /* bytes resp. words between rows, 0: shared by all rows */
+  int32_t history_dtype;         /* M355_I64 / M355_I32 */
+  int32_t bias_dtype;            /* the dtype of the logits, or M355_F32 with F16 / BF16 logits */
+  int32_t mask_kind;             /* m355_mask_kind */
+  int32_t reserved;
+  m355_operand repetition, presence, frequency, temperature;
+} m355_logit_adjust;
+int m355_logits_adjust(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
+                       const m355_logit_adjust* adjust, void* out, int64_t out_stride, void* stream);
+/*
+ * The gradient of m355_logits_adjust: for g = d L / d s,
+ *     dlogits = allowed ? g / temperature * (c_all > 0 ? (z > 0 ? 1 / repetition : repetition) : 1) : 0
+ *     dbias   = allowed ? g / temperature : 0, per element (bias_stride != 0: rows x k contiguous values of bias_dtype)
+ *               or summed over the rows in a fixed order, in float64 (bias_stride == 0: k values)
+ * dlogits (rows x k contiguous) or dbias may be NULL: not wanted.  logits is read only with a history.  workspace:
+ * m355_logits_adjust_grad_workspace_bytes bytes, 8-byte aligned, needed with dbias and bias_stride 0; scratch.
+ */
+size_t m355_logits_adjust_grad_workspace_bytes(int64_t rows, int64_t k, int dtype);
+int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const void* g, int64_t g_stride, const void* logits,
+                            int64_t logits_stride, const m355_logit_adjust* adjust, void* dlogits, void* dbias,
+                            void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * out[r] = log-density of observation x[r] (M355_I64 / I32 / F64 / F32) under row r: z[x] - log sum exp(z).  -inf when x
+ * is not an integer in [0, k) or when every logit of the row is -inf; NaN when the row holds NaN or +inf.
+ * workspace: m355_logits_workspace_bytes bytes, 8-byte aligned, scratch; calls that may run concurrently need one each.
+ */
+size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype);
+int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride, const void* x,
+                       int x_dtype, void* out, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * total = sum_r w_r logpdf_r (added in float64, in a fixed order) and, unless dlogits is NULL, its gradient
+ *     dlogits[r, v] = w_r ((v == x_r) - exp(z_v) / sum exp(z))   (dtype; 0 where x_r is no category or the whole row is -inf)
+ * weights: operand over the row index (float64 / float32 array or scalar).  A row of weight 0 contributes 0 and gets
+ * gradient 0, whatever it holds.  dlogits may be the logits themselves (same address and stride); any other overlap with
+ * an input is undefined.
+ */
+int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
+                                const void* x, int x_dtype, const m355_operand* weights, void* total, void* dlogits,
+                                int64_t dlogits_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * 2-norm over a list of tensors (M355_F64 / F32 / F16 / BF16 each, n contiguous elements of any alignment) and clipping
+ * by it.  `tensors` is a HOST array, read during the call only.
+ *   m355_global_norm       norm = sqrt(sum of all squares), the squares added in float64 in a fixed order; *sumsq (device,
+ *                          or NULL) receives the sum, norm (device, norm_dtype F64 / F32, or NULL) its square root
+ *   m355_clip_global_norm  out = norm > max_norm ? ptr * (max_norm / norm) : ptr, per tensor, one rounding; a norm that is
+ *                          not finite scales nothing.  sumsq (device, one double) replaces the sum over `tensors` where it
+ *                          is not NULL (a sum over the shards of several processes).  norm as above.
+ * out may be ptr itself; M355_ERR_INVALID if an output overlaps another tensor's memory.  workspace:
+ * m355_global_norm_workspace_bytes(count) bytes, 8-byte aligned, scratch; calls that may run concurrently need one each.
+ */
+typedef struct m355_tensor {
+  const void* ptr;
+  void* out; /* m355_clip_global_norm only */
+  int64_t n;
+  int32_t dtype;
+  int32_t reserved;
+} m355_tensor;
+size_t m355_global_norm_workspace_bytes(int64_t count);
+int m355_global_norm(int64_t count, const m355_tensor* tensors, double* sumsq, void* norm, int norm_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int m355_clip_global_norm(int64_t count, const m355_tensor* tensors, double max_norm, const double* sumsq, void* norm,
+                          int norm_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

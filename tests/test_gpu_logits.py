@@ -1,0 +1,573 @@
+"""Categorical given by logits on the GPU: adjustment and its gradient, log-density, weighted sum and its gradient, against
+plain float64 implementations.  Tolerances are worst-case bounds counted from the roundings of the formulas: u is half a
+step of the arithmetic (2^-24, float64: 2^-53), ut half a step of the storage type."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+INF = math.inf
+
+
+def steps(dtype):
+    """(u, ut, half the smallest subnormal) of a storage type."""
+    u = 2.0**-53 if dtype == torch.float64 else 2.0**-24
+    info = torch.finfo(dtype)
+    return u, info.eps / 2, info.tiny * info.eps / 2
+
+
+def within(got, ref, bound):
+    """|got - ref| <= bound where ref is finite; the same infinities and NaN elsewhere."""
+    got, ref = got.detach().cpu().double(), ref.double()
+    assert got.shape == ref.shape
+    fin = ref.isfinite()
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got[~fin & ~ref.isnan()], ref[~fin & ~ref.isnan()])
+    d = (got[fin] - ref[fin]).abs()
+    b = bound.expand(ref.shape)[fin] if isinstance(bound, torch.Tensor) else torch.full_like(d, bound)
+    assert bool((d <= b).all()), f"worst {float((d / b.clamp(min=1e-300)).max()):.3g} times the bound"
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def allowed_of(mask, k, rows):
+    if mask is None:
+        return torch.ones(rows, k, dtype=torch.bool)
+    m = mask.cpu()
+    if m.dtype == torch.int32:
+        v = torch.arange(k)
+        m = (m.long()[..., v // 32] >> (v % 32)) & 1 == 1
+    return m.reshape(-1, k).expand(rows, k)
+
+
+def per_row(a, rows):
+    return torch.as_tensor(a, dtype=torch.float64).cpu().reshape(-1).expand(rows)
+
+
+def counts_of(history, lengths, prompts, rows, k):
+    call = torch.zeros(rows, k, dtype=torch.float64)
+    cgen = torch.zeros(rows, k, dtype=torch.float64)
+    if history is None:
+        return call, cgen
+    h = history.cpu().long().reshape(-1, history.shape[-1]).expand(rows, -1)
+    n = h.shape[1]
+    for r in range(rows):
+        last = n if lengths is None else max(0, min(n, int(lengths.reshape(-1)[r])))
+        first = 0 if prompts is None else int(prompts.reshape(-1)[r])
+        for i in range(last):
+            v = int(h[r, i])
+            if 0 <= v < k:
+                call[r, v] += 1
+                cgen[r, v] += i >= first
+    return call, cgen
+
+
+def plain_adjust(z, history=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
+                 temperature=1.0, mask=None):
+    """(result, bound on the error) in float64."""
+    dtype = z.dtype
+    u, ut, tiny = steps(dtype)
+    k = z.shape[-1]
+    x = z.cpu().double().reshape(-1, k)
+    rows = x.shape[0]
+    call, cgen = counts_of(history, lengths, prompt_lengths, rows, k)
+    rep, pres, freq, t = (per_row(a, rows)[:, None] for a in (repetition, presence, frequency, temperature))
+    s = torch.where(call > 0, torch.where(x > 0, x / rep, x * rep), x)
+    size = s.abs() + freq.abs() * cgen + pres.abs() * (cgen > 0)
+    s = s - (freq * cgen + pres * (cgen > 0))
+    if bias is not None:
+        b = bias.cpu().double().reshape(-1, k).expand(rows, k)
+        s = s + b
+        size = size + b.abs()
+    ok = allowed_of(mask, k, rows)
+    ref = torch.where(ok, s / t, -INF)
+    # roundings before the last: rep, x / rep, freq, freq * c, pres, their sum, the difference, the sum with the bias, 1 / T,
+    # its product: 10, each at most u times `size` / T (times 1 + a few u: 12)
+    bound = ut * ref.abs() + 12 * u * size / t.abs() + tiny
+    return ref.reshape(z.shape), torch.nan_to_num(bound, nan=0.0, posinf=0.0).reshape(z.shape)
+
+
+def plain_adjust_grad(g, z, history=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
+                      bias=None, temperature=1.0, mask=None):
+    k = z.shape[-1]
+    x, gg = z.cpu().double().reshape(-1, k), g.cpu().double().reshape(-1, k)
+    rows = x.shape[0]
+    call, _ = counts_of(history, lengths, prompt_lengths, rows, k)
+    rep, t = (per_row(a, rows)[:, None] for a in (repetition, temperature))
+    ok = allowed_of(mask, k, rows)
+    db = torch.where(ok, gg / t, 0.0)
+    dz = torch.where(ok & (call > 0), torch.where(x > 0, db / rep, db * rep), db)
+    return dz.reshape(z.shape), db
+
+
+def plain_logpdf(x, z, weights=None):
+    """log-densities, total and gradient in float64 with their bounds."""
+    dtype = z.dtype
+    u, ut, tiny = steps(dtype)
+    k = z.shape[-1]
+    zz = z.cpu().double().reshape(-1, k)
+    rows = zz.shape[0]
+    xx = torch.as_tensor(x).cpu().double().reshape(-1).expand(rows)
+    w = torch.ones(rows, dtype=torch.float64) if weights is None else torch.as_tensor(weights).cpu().double().reshape(-1).expand(rows)
+    m = zz.max(dim=1, keepdim=True).values
+    mm = torch.where(m == -INF, 0.0, m)
+    e = (zz - mm).exp()
+    s = e.sum(dim=1, keepdim=True)
+    inside = (xx >= 0) & (xx < k) & (xx == xx.floor())
+    xi = torch.where(inside, xx, 0.0).long()[:, None]
+    zx = zz.gather(1, xi)
+    empty = (s == 0)[:, 0]
+    lp = torch.where(inside & ~empty, (zx - mm - s.log())[:, 0], -INF)
+    # sum of k terms, one after the other at worst over a 64th of the row, then joined: k / 64 + 24 roundings; exp 2^-22
+    # (float64: 2^-50) and the rounding of z - m, which moves the exponent by u |z - m|: weighted by p, at most
+    # u * sum(p |z - m|); log: 2 u |log s|; the two differences: u each
+    p = torch.where(s > 0, e / s, 0.0)
+    spread = torch.nan_to_num((p * (zz - mm).abs()).sum(1), nan=0.0, posinf=0.0)
+    off_s = (k / 64 + 24) * u + 4 * u + 4 * u * spread
+    finite = lambda t: torch.nan_to_num(t, nan=0.0, posinf=0.0, neginf=0.0).abs()  # noqa: E731
+    b_lp = 1.01 * off_s + 2 * u * finite(s.log()[:, 0]) + u * finite((zx - mm)[:, 0]) + 2 * u * finite(lp)
+    grad = torch.zeros(rows, k, dtype=torch.float64)
+    live = (w != 0) & inside & ~empty
+    hot = torch.zeros(rows, k, dtype=torch.float64).scatter_(1, xi, 1.0)
+    grad = torch.where(live[:, None], w[:, None] * (hot - p), 0.0)
+    d = torch.nan_to_num((zz - mm).abs(), nan=0.0, posinf=0.0)
+    rel_p = 4 * u + 4 * u * d + (1.01 * off_s + 4 * u)[:, None]
+    floor = 2.0**-125 if dtype != torch.float64 else 2.0**-1000  # where exp is flushed
+    b_g = ut * finite(grad) + finite(w)[:, None] * (finite(p) * rel_p + 2 * u * hot + floor) + tiny
+    terms = torch.where(w == 0, 0.0, w * lp)
+    total = terms.sum()
+    b_total = float((finite(w) * b_lp).sum() + 2 * u * finite(terms).sum())
+    shape = z.shape[:-1]
+    return lp.reshape(shape), b_lp.reshape(shape), total, b_total, grad.reshape(z.shape), b_g.reshape(z.shape)
+
+
+def make(shape, dtype, seed, device, scale=3.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * scale).to(dtype).to(device)
+
+
+# ----------------------------------------------------------------------------------------------------- adjust
+SIZES = [(1, 1), (1, 2), (3, 7), (2, 33), (5, 64), (3, 1023), (2, 4097), (2, 8192), (3, 20011)]
+
+
+def adjust_args(rows, k, seed, device, history=37, mask="bool", bias="shared", wide=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda lo, hi: (lo + (hi - lo) * torch.rand(rows, generator=gen, dtype=torch.float64)).to(wide).to(device)  # noqa: E731
+    a = dict(temperature=r(0.5, 2.0))
+    if history:
+        h = torch.randint(-2, max(2, min(k + 2, 50)), (rows, history), generator=gen)
+        h[:, ::5] = torch.randint(0, k, h[:, ::5].shape, generator=gen)
+        a.update(history=h.to(device), lengths=torch.randint(-1, history + 3, (rows,), generator=gen).to(device),
+                 prompt_lengths=torch.randint(0, history + 1, (rows,), generator=gen).to(device) // 2,
+                 repetition=r(0.8, 1.5), presence=r(-0.5, 1.0), frequency=r(-0.2, 0.5))
+    if bias:
+        shape = (k,) if bias == "shared" else (rows, k)
+        a["bias"] = torch.randn(*shape, generator=gen, dtype=torch.float64).to(wide).to(device)
+    if mask:
+        ok = torch.rand(rows, k, generator=gen) < 0.6
+        ok[-1] = False  # a row that allows nothing
+        if mask == "bits":
+            words = (k + 31) // 32
+            bits = torch.zeros(rows, words * 32, dtype=torch.int64)
+            bits[:, :k] = ok
+            w = (bits.reshape(rows, words, 32) << torch.arange(32)).sum(2)
+            ok = torch.where(w >= 2**31, w - 2**32, w).to(torch.int32)
+        a["mask"] = ok.to(device)
+    return a
+
+
+@pytest.mark.parametrize("rows, k", SIZES)
+@pytest.mark.parametrize("dt", DT)
+def test_adjust_and_its_gradient(gpu, dt, rows, k):
+    from distributions_amd import categorical_logits as cl
+
+    dtype = DT[dt]
+    wide = torch.float64 if dt == "f64" else torch.float32
+    u, ut, tiny = steps(dtype)
+    z, g = make((rows, k), dtype, 1, gpu), make((rows, k), dtype, 2, gpu)
+    for i, (mask, bias, history) in enumerate([("bool", "shared", 37), ("bits", "rows", 300), (None, None, 5), ("bits", "shared", 0),
+                                               ("bool", None, 0), (None, "rows", 0)]):
+        a = adjust_args(rows, k, 10 + i, gpu, history, mask, bias, wide)
+        ref, bound = plain_adjust(z, **a)
+        out = cl.adjust(z, **a)
+        assert out.dtype == dtype
+        within(out, ref, bound)
+        dz, db = cl.adjust_grad(g, z, **a)
+        rz, rb = plain_adjust_grad(g, z, **a)
+        # 1 / T, its product, rep, its product or quotient: 4 roundings
+        within(dz, rz, ut * rz.abs() + 6 * u * rz.abs() + tiny)
+        if bias is None:
+            assert db is None
+        elif bias == "rows":
+            within(db, rb, 3 * u * rb.abs() + 2.0**-149)
+        else:  # added in float64; the result rounded to float32 (u) again
+            within(db, rb.sum(0), 4 * u * rb.abs().sum(0) + 2.0**-149)
+    same = [cl.adjust(z, **a) for _ in range(2)] + [cl.adjust_grad(g, z, **a)[1] for _ in range(2)]
+    assert torch.equal(same[0], same[1]) and torch.equal(same[2], same[3])
+
+
+def test_adjust_infinities_nan_and_lowest_values(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    for dtype in DT.values():
+        low = torch.finfo(dtype).min
+        z = torch.tensor([[0.0, -0.0, INF, -INF, math.nan, low, -low, 1.0, -1.0]] * 2, dtype=dtype, device=gpu)
+        ok = torch.tensor([[True] * 9, [True, True, False, True, False, True, False, False, True]], device=gpu)
+        h = torch.tensor([[0, 1, 2, 3, 5, 8, 8, 9, -1]] * 2, device=gpu)
+        a = dict(history=h, repetition=2.0, mask=ok)
+        ref, bound = plain_adjust(z, **a)
+        ref = ref.to(dtype).double()  # lowest * 2 leaves the type
+        out = cl.adjust(z, **a)
+        within(out, ref, bound)
+        # NaN and infinities of g where nothing is allowed stay out of the gradient
+        g = torch.where(ok, torch.ones_like(z), torch.full_like(z, math.nan))
+        dz, db = cl.adjust_grad(g, z, bias=torch.zeros(9, dtype=dtype, device=gpu), **a)
+        assert bool(dz.isfinite().all()) and bool(db.isfinite().all())
+        assert bool((dz[1][~ok[1]] == 0).all())
+        # x <= 0 takes the branch of the product: at 0 the slope is `repetition`
+        assert float(dz[0, 0]) == 2.0 and float(dz[0, 2]) == 0.5 and float(dz[0, 8]) == 2.0 and float(dz[0, 7]) == 1.0
+        lowest = torch.full((9,), low, dtype=dtype, device=gpu)  # a mask spelled as the type's lowest value
+        within(cl.adjust(torch.ones(1, 9, dtype=dtype, device=gpu), bias=lowest), torch.full((1, 9), low, dtype=torch.float64), abs(low) * 2.0**-7)
+
+
+def test_adjust_long_and_degenerate_histories(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    k = 300
+    z = make((3, k), torch.float32, 3, gpu)
+    one = torch.zeros(3, 5000, dtype=torch.int32, device=gpu)  # one token, 5000 times
+    lengths = torch.tensor([5000, 1, 0], device=gpu)
+    a = dict(history=one, lengths=lengths, frequency=0.01, presence=0.5, repetition=1.3)
+    ref, bound = plain_adjust(z, **a)
+    within(cl.adjust(z, **a), ref, bound)
+    shared = torch.arange(k, device=gpu)[None, :].expand(3, k)  # a history all rows share, without a copy
+    a = dict(history=shared, repetition=1.7)
+    ref, bound = plain_adjust(z, **a)
+    within(cl.adjust(z, **a), ref, bound)
+    far = torch.tensor([[2**40, -(2**40), 2**32, k, -k, 0]], device=gpu)  # ids that are no categories, also modulo 2^32
+    a = dict(history=far, presence=1.0)
+    ref, bound = plain_adjust(z, **a)
+    within(cl.adjust(z, **a), ref, bound)
+    a = dict(history=torch.zeros(3, 0, dtype=torch.int64, device=gpu), presence=1.0, repetition=2.0)
+    assert torch.equal(cl.adjust(z, **a), z)
+    assert cl.adjust(z[:0], temperature=2.0).shape == (0, k)
+
+
+def strided(z):
+    """The same values in other layouts: odd offset, row gap, transposed, last of three axes, expanded."""
+    rows, k = z.shape
+    big = torch.full((rows, k + 5), 7.0, dtype=z.dtype, device=z.device)
+    big[:, 3 : 3 + k] = z
+    yield big[:, 3 : 3 + k]
+    yield z.t().contiguous().t()
+    cube = torch.full((rows, 3, k), 7.0, dtype=z.dtype, device=z.device)
+    cube[:, 2] = z
+    yield cube[:, 2, :]
+    flat = torch.full((rows * k + 1,), 7.0, dtype=z.dtype, device=z.device)
+    flat[1:] = z.reshape(-1)
+    yield flat[1:].reshape(rows, k)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_layouts(gpu, dt):
+    from distributions_amd import categorical_logits as cl
+
+    rows, k = 4, 1021
+    z = make((rows, k), DT[dt], 5, gpu)
+    x = torch.tensor([0, 1020, -1, 77], device=gpu)
+    w = torch.tensor([1.0, 0.5, 2.0, -1.0], device=gpu)
+    a = adjust_args(rows, k, 6, gpu, wide=torch.float64 if dt == "f64" else torch.float32)
+    want, lp = cl.adjust(z, **a), cl.logpdf(x, z)
+    total, (_, grad) = cl.sum_logpdf_grad(x, z, w)
+    dz, db = cl.adjust_grad(z, z, **a)
+    for y in strided(z):
+        assert torch.equal(cl.adjust(y, **a), want)
+        assert torch.equal(cl.logpdf(x, y), lp)
+        t2, (_, g2) = cl.sum_logpdf_grad(x, y, w)
+        assert torch.equal(t2, total) and torch.equal(g2, grad)
+        got = cl.adjust_grad(y, y, **a)
+        assert torch.equal(got[0], dz) and torch.equal(got[1], db)
+    # leading axes; arguments that broadcast along some of them
+    y = z.reshape(2, 2, k)
+    assert torch.equal(cl.logpdf(x.reshape(2, 2), y), lp.reshape(2, 2))
+    t = torch.tensor([[0.5], [2.0]], device=gpu)
+    assert torch.equal(cl.adjust(y, temperature=t)[1], cl.adjust(y[1], temperature=2.0))
+    bias = make((2, 1, k), torch.float32, 8, gpu) if dt != "f64" else make((2, 1, k), torch.float64, 8, gpu)
+    _, db = cl.adjust_grad(y, y, bias=bias, temperature=t)
+    ref = (y.cpu().double() / t.cpu().double()[:, :, None]).sum(1, keepdim=True)
+    size = (y.cpu().double().abs() / t.cpu().double()[:, :, None]).sum(1, keepdim=True)
+    u = steps(bias.dtype)[0]
+    within(db, ref, 6 * u * size)
+    one = cl.logpdf(77, z[3])
+    assert one.shape == () and torch.equal(one, lp[3])
+    assert torch.equal(cl.logpdf(77, z[3:4].expand(5, k)), lp[3].expand(5))
+
+
+def test_out_in_place(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    for dtype in (torch.bfloat16, torch.float32, torch.float64):
+        z = make((6, 5003), dtype, 9, gpu)
+        a = adjust_args(6, 5003, 11, gpu, wide=torch.float64 if dtype == torch.float64 else torch.float32)
+        want = cl.adjust(z, **a)
+        y = z.clone()
+        assert cl.adjust(y, out=y, **a) is y and torch.equal(y, want)
+        pad = torch.full((6, 5010), 7.0, dtype=dtype, device=gpu)
+        cl.adjust(z, out=pad[:, 2:5005], **a)
+        assert torch.equal(pad[:, 2:5005], want) and bool((pad[:, :2] == 7).all()) and bool((pad[:, 5005:] == 7).all())
+        x = torch.tensor([0, 5002, 3, -1, 7, 2500], device=gpu)
+        total, (_, grad) = cl.sum_logpdf_grad(x, z)
+        y = z.clone()
+        t2, (_, g2) = cl.sum_logpdf_grad(x, y, out=y)
+        assert g2 is y and torch.equal(y, grad) and torch.equal(t2, total)
+
+
+# ------------------------------------------------------------------------------------------------- log-density
+@pytest.mark.parametrize("rows, k", SIZES + [(2, 50021), (1, 131072), (1, 262147), (300, 515), (700, 64)])
+@pytest.mark.parametrize("dt", DT)
+def test_logpdf_total_and_gradient(gpu, dt, rows, k):
+    from distributions_amd import categorical_logits as cl
+
+    dtype = DT[dt]
+    z = make((rows, k), dtype, k + rows, gpu)
+    gen = torch.Generator().manual_seed(k)
+    x = torch.randint(0, k, (rows,), generator=gen)
+    w = torch.randn(rows, generator=gen, dtype=torch.float64 if dt == "f64" else torch.float32)
+    if rows > 2:
+        x[1], w[2] = -1, 0.0
+    lp, b_lp, total, b_total, grad, b_g = plain_logpdf(x, z, w)
+    got = cl.logpdf(x.to(gpu), z)
+    assert got.dtype == (torch.float64 if dt == "f64" else torch.float32)
+    within(got, lp, b_lp)
+    w0 = torch.where(x < 0, 0.0, w)  # -inf would swallow the total
+    _, _, total, b_total, _, _ = plain_logpdf(x, z, w0)
+    within(cl.sum_logpdf(x.to(gpu), z, w0.to(gpu)), total, b_total)
+    t, (none, g) = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    assert none is None and g.dtype == dtype
+    within(g, grad, b_g)
+    t, _ = cl.sum_logpdf_grad(x.to(gpu), z, w0.to(gpu))
+    within(t, total, b_total)
+    again = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    assert torch.equal(again[1][1], g)
+
+
+@pytest.mark.parametrize("k", [3, 700, 70001])
+@pytest.mark.parametrize("dt", DT)
+def test_rows_without_a_finite_answer(gpu, dt, k):
+    from distributions_amd import categorical_logits as cl
+
+    dtype = DT[dt]
+    z = make((8, k), dtype, 4, gpu)
+    z[0] = -INF  # nothing left
+    z[1, 1:] = -INF  # one category left
+    z[2, 2] = math.nan
+    z[3, 0] = INF
+    z[4] = torch.finfo(dtype).min  # a mask spelled as the lowest value: uniform
+    z[5, 0] = -torch.finfo(dtype).min  # the largest value next to small ones
+    z[6] = math.nan  # padding
+    z[7, 2] = -INF  # the observation is not allowed, others are
+    x = torch.tensor([1, 0, 0, 0, 2, 0, 1, 2], device=gpu)
+    w = torch.tensor([1.0, 1, 1, 1, 1, 1, 0, 1], device=gpu)
+    lp = cl.logpdf(x, z).cpu().double()
+    assert lp[0] == -INF and lp[1] == 0 and lp[2].isnan() and lp[3].isnan() and lp[6].isnan() and lp[7] == -INF
+    assert abs(float(lp[4]) + math.log(k)) <= 1e-4 * math.log(k) and lp[5] == 0
+    total, (_, g) = cl.sum_logpdf_grad(x, z, w)
+    g = g.cpu().double()
+    assert total.isnan()
+    assert bool((g[0] == 0).all()) and bool((g[1] == 0).all()) and bool(g[2].isnan().all()) and bool(g[3].isnan().all())
+    assert bool((g[6] == 0).all())
+    *_, ref, b = plain_logpdf(x[4:], z[4:], w[4:])
+    within(g[4:], ref, b)
+    keep = torch.tensor([0.0, 1, 0, 0, 1, 1, 0, 0], device=gpu)
+    assert bool(cl.sum_logpdf(x, z, keep).isfinite())
+    # labels that are no category, in every type they may have
+    for bad in ([-1, k, k + 5, -(2**40)], [-1.0, float(k), 0.5, math.nan]):
+        xb = torch.tensor(bad * 2, device=gpu)
+        assert bool((cl.logpdf(xb, z[5:6].expand(8, k)) == -INF).all())
+        t, (_, g) = cl.sum_logpdf_grad(xb, z[5:6].expand(8, k))
+        assert t == -INF and bool((g == 0).all())
+    for good in (torch.int32, torch.int64, torch.float32, torch.float64, torch.int16):
+        assert torch.equal(cl.logpdf(torch.tensor([2], device=gpu).to(good), z[5:6]), cl.logpdf(2, z[5:6]))
+
+
+def test_gradients_against_differences(gpu):
+    """The whole chain adjust -> sum_logpdf in float64 against central differences, leaf by leaf."""
+    from distributions_amd import categorical_logits as cl
+
+    rows, k = 3, 11
+    z = make((rows, k), torch.float64, 20, gpu, 1.0)
+    a = adjust_args(rows, k, 21, gpu, 9, None, "shared", torch.float64)
+    x = torch.tensor([1, 5, 10], device=gpu)
+    w = torch.tensor([1.0, 0.3, 2.0], dtype=torch.float64, device=gpu)
+
+    def f(zz, bias):
+        return float(cl.sum_logpdf(x, cl.adjust(zz, **{**a, "bias": bias}), w))
+
+    _, (_, g) = cl.sum_logpdf_grad(x, cl.adjust(z, **a), w)
+    dz, db = cl.adjust_grad(g, z, **a)
+    h = 1e-5  # error h^2 / 6 times a third derivative below 10, and 2^-52 |f| / h
+    for i in range(rows):
+        for j in range(k):
+            if abs(float(z[i, j])) < 2 * h:
+                continue  # the kink of the repetition penalty
+            e = torch.zeros_like(z)
+            e[i, j] = h
+            assert abs((f(z + e, a["bias"]) - f(z - e, a["bias"])) / (2 * h) - float(dz[i, j])) < 1e-8
+    for j in range(k):
+        e = torch.zeros_like(a["bias"])
+        e[j] = h
+        assert abs((f(z, a["bias"] + e) - f(z, a["bias"] - e)) / (2 * h) - float(db[j])) < 1e-8
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows 2^31 elements apart: the third starts 2^32 elements behind the first."""
+    from distributions_amd import categorical_logits as cl
+
+    k = 1000
+    flat = torch.empty(2**32 + k, dtype=torch.bfloat16, device=gpu)
+    z = flat.as_strided((3, k), (2**31, 1))
+    z.copy_(make((3, k), torch.bfloat16, 30, gpu))
+    small = z.contiguous()
+    x = torch.tensor([0, 999, 500], device=gpu)
+    a = adjust_args(3, k, 31, gpu)
+    assert torch.equal(cl.logpdf(x, z), cl.logpdf(x, small))
+    assert torch.equal(cl.adjust(z, **a), cl.adjust(small, **a))
+    total, (_, g) = cl.sum_logpdf_grad(x, small)
+    t2, _ = cl.sum_logpdf_grad(x, z, out=z)
+    assert torch.equal(total, t2) and torch.equal(z, g)
+
+
+def test_numpy_and_types(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    z = np.random.default_rng(0).normal(size=(4, 9))
+    lp = cl.logpdf([0, 1, 2, 9], z)
+    assert isinstance(lp, np.ndarray) and lp.dtype == np.float64 and np.isneginf(lp[3])
+    ref = z - np.log(np.exp(z).sum(1, keepdims=True))
+    assert np.allclose(lp[:3], ref[[0, 1, 2], [0, 1, 2]], rtol=1e-13)
+    total, (none, g) = cl.sum_logpdf_grad([0, 1, 2, 3], z)
+    assert isinstance(total, float) and none is None and g.shape == z.shape
+    assert np.allclose(g, np.eye(9)[:4] - np.exp(ref), atol=1e-14)
+    out = cl.adjust(z.astype(np.float32), history=[[1, 1]] * 4, frequency=0.5, mask=np.arange(9) < 5)
+    assert out.dtype == np.float32 and np.isneginf(out[:, 5:]).all()
+    assert np.allclose(out[:, 1], z[:, 1].astype(np.float32) - 1.0, atol=1e-6)
+    assert cl.logpdf(1, [0, 0, 0]).dtype == np.float64  # integers become float64
+
+
+def test_refusals(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    z = make((4, 10), torch.float32, 1, gpu)
+    h = torch.zeros(4, 3, dtype=torch.int64, device=gpu)
+    bad = [
+        (ValueError, dict(repetition=0.0, history=h)), (ValueError, dict(temperature=-1.0)), (ValueError, dict(repetition=1.2)),
+        (ValueError, dict(presence=0.1)), (ValueError, dict(lengths=h[:, 0])), (TypeError, dict(history=h.float())),
+        (ValueError, dict(history=h[:3])), (ValueError, dict(history=h, lengths=h[:3, 0])), (TypeError, dict(history=h, lengths=z[:, 0])),
+        (ValueError, dict(bias=z[:, :9])), (ValueError, dict(bias=z[:3])), (TypeError, dict(mask=z)), (ValueError, dict(mask=z[:, :9] > 0)),
+        (ValueError, dict(mask=h[:, :2].int())), (ValueError, dict(temperature=z[:3, 0])), (ValueError, dict(out=z[:3])),
+        (ValueError, dict(out=z.double())), (ValueError, dict(out=z.t().contiguous().t())), (ValueError, dict(out=z[:1].expand(4, 10))),
+        (ValueError, dict(out=torch.empty(8, 10, device=gpu)[::2], bias=None, mask=None, temperature=z.new_ones(3))),
+    ]
+    for err, kw in bad:
+        with pytest.raises(err):
+            cl.adjust(z, **kw)
+    buf = torch.zeros(5, 10, device=gpu)
+    with pytest.raises(ValueError, match="overlaps"):
+        cl.adjust(buf[:4], out=buf[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        cl.adjust(z, bias=buf[:4], out=buf[:4])
+    with pytest.raises(ValueError):
+        cl.adjust_grad(z[:, :9], z)
+    with pytest.raises(ValueError):
+        cl.logpdf(torch.zeros(3, device=gpu), z)
+    with pytest.raises(ValueError):
+        cl.logpdf(0, torch.zeros(3, 0, device=gpu))
+    with pytest.raises(TypeError):
+        cl.logpdf(0, z.to(torch.complex64))
+    with pytest.raises(ValueError):
+        cl.sum_logpdf(0, z, torch.ones(3, device=gpu))
+
+
+# --------------------------------------------------------------------------- runs of them together, streams, graphs
+def step(z, x, w, a, max_norm):
+    """A training step of a constrained categorical: adjust, log-density, its gradient, back through adjust, clip."""
+    from distributions_amd import categorical_logits as cl
+    from distributions_amd import gradients
+
+    s = cl.adjust(z, **a)
+    total, (_, g) = cl.sum_logpdf_grad(x, s, w)
+    dz, db = cl.adjust_grad(g, z, **a)
+    norm, (dz, db) = gradients.clip_global_norm([dz, db], max_norm)
+    return total, norm, dz, db
+
+
+@pytest.mark.parametrize("dt", ["f64", "f32", "bf16"])
+def test_step_against_autograd(gpu, dt):
+    rows, k = 40, 2003
+    dtype = DT[dt]
+    wide = torch.float64 if dt == "f64" else torch.float32
+    u, ut, _ = steps(dtype)
+    z = make((rows, k), dtype, 40, gpu, 1.5)
+    a = adjust_args(rows, k, 41, gpu, 25, "bool", "shared", wide)
+    a["mask"][:] = True
+    a["mask"][:, ::7] = False
+    x = torch.arange(rows, device=gpu) * 7 + 1
+    w = torch.ones(rows, dtype=wide, device=gpu)
+    w[::6] = 0
+    total, norm, dz, db = step(z, x, w, a, 0.5)
+    zr = z.cpu().double().requires_grad_()
+    br = a["bias"].cpu().double().requires_grad_()
+    call, cgen = counts_of(a["history"], a["lengths"], a["prompt_lengths"], rows, k)
+    p = {n: a[n].cpu().double()[:, None] for n in ("repetition", "presence", "frequency", "temperature")}
+    s = torch.where(call > 0, torch.where(zr > 0, zr / p["repetition"], zr * p["repetition"]), zr)
+    s = (s - p["frequency"] * cgen - p["presence"] * (cgen > 0) + br) / p["temperature"]
+    s = s.masked_fill(~a["mask"].cpu(), -INF)
+    ref = (w.cpu().double() * (s.gather(1, x.cpu()[:, None])[:, 0] - torch.logsumexp(s, 1))).sum()
+    ref.backward()
+    n = torch.sqrt(zr.grad.square().sum() + br.grad.square().sum())
+    # logits between -20 and 20 are rounded once on the way (20 ut each), gradients twice: relative to the whole
+    tol = 40 * ut + 4000 * u
+    assert abs(float(total) - float(ref)) <= tol * rows
+    assert abs(float(norm) - float(n)) <= tol * float(n)
+    f = 0.5 / float(n)
+    assert float((dz.cpu().double() - zr.grad * f).norm()) <= tol * 0.5
+    assert float((db.cpu().double() - br.grad * f).norm()) <= tol * 0.5
+
+
+def test_streams_and_captured_graphs(gpu):
+    """A step on another stream, and two captured graphs of it replayed in turn with eager work in between."""
+    rows, k = 33, 5003
+    z = make((rows, k), torch.bfloat16, 50, gpu)
+    a = adjust_args(rows, k, 51, gpu, 40, "bits", "shared")
+    a["mask"][-1] = -1
+    x = torch.arange(rows, device=gpu)
+    w = torch.ones(rows, device=gpu)
+    want = step(z, x, w, a, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(z, x, w, a, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    graphs = []
+    for max_norm in (0.1, 1e9):
+        with torch.cuda.stream(side):
+            step(z, x, w, a, max_norm)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step(z, x, w, a, max_norm)
+        graphs.append((graph, res, max_norm))
+    for i in range(4):
+        z.copy_(make((rows, k), torch.bfloat16, 60 + i, gpu))
+        for graph, res, max_norm in graphs:
+            for r in res:
+                r.fill_(7)
+            graph.replay()
+            torch.cuda.synchronize()
+            eager = step(z, x, w, a, max_norm)
+            assert all(torch.equal(p, q) for p, q in zip(res, eager)), (i, max_norm)
