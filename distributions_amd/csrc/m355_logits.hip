@@ -217,14 +217,11 @@ __global__ __launch_bounds__(kAdjThreads) void k_logits_cols_final(const double*
 }
 
 // ----------------------------------------------------------------------------------------- log-density
-// exp(d) for d <= 0 (d > 0 only where the row holds +inf): 2^(d log2 e) with the product's rounding error carried along,
-// relative error below 2^-22 wherever the result is a normal float, 0 below; NaN stays NaN.
-M355_DEV float exp_neg(float d) {
-  const float t = d * 1.44269502f;                              // float(log2 e)
-  const float r = __builtin_fmaf(d, 1.44269502f, -t) + d * 1.92596303e-8f;  // log2 e - float(log2 e)
-  const float p = __builtin_amdgcn_exp2f(t);
-  return d < -87.0f ? 0.0f : __builtin_fmaf(p, r * 0.693147182f, p);
-}
+// exp(d) for d <= 0 or NaN (d = z - maximum): 2^(d log2 e).  The roundings of d, of log2 e and of their product move the
+// exponent by less than 3 * 2^-24 |d|: a large |d| has a small exp(d), so the sum of a row keeps 2^-22 or so, and exp(0) is
+// 1.  Results below 2^-126 are 0.  (One fused multiply-add from z to the exponent saves an operation per element and no
+// time, and the maximum's own exp is then off 1 by the rounding of its product.)
+M355_DEV float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502f); }
 M355_DEV double exp_neg(double d) { return ::exp(d); }
 M355_DEV float log_c(float v) { return ::logf(v); }
 M355_DEV double log_c(double v) { return ::log(v); }
@@ -264,81 +261,271 @@ template <class C> M355_DEV void join(C& m, C& s, C m2, C s2) {
   m = mm;
 }
 
-template <class T> M355_DEV void accumulate(const typename T::comp (&z)[kPer<T>], typename T::comp& m, typename T::comp& s) {
-  typedef typename T::comp comp;
-  comp mv = z[0];
-#pragma unroll
-  for (int e = 1; e < kPer<T>; ++e) mv = max_c(mv, z[e]);
-  if (mv > m) {
-    s *= exp_neg(m - mv);  // m = -inf: 0
-    m = mv;
-  }
-  const comp b = finite_max(m);
-#pragma unroll
-  for (int e = 0; e < kPer<T>; ++e) s += exp_neg(z[e] - b);
-}
-
-template <int THREADS, class C> M355_DEV void block_join(C& m, C& s) {
-  __shared__ C red[2][THREADS / 64];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) join<C>(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (lane == 0) {
-    red[0][wave] = m;
-    red[1][wave] = s;
-  }
-  __syncthreads();
-  m = red[0][0];
-  s = red[1][0];
-#pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) join<C>(m, s, red[0][w], red[1][w]);
-  __syncthreads();
-}
-
 // log-density from the row's statistics; -inf for an observation that is no category and for a row that is all -inf
 template <class C> M355_DEV C density(C zx, C m, C s, bool inside) {
   return !inside || s == (C)0 ? (C)-kInf : (zx - finite_max(m)) - log_c(s);
 }
 
-// One workgroup per row: one pass for the running maximum and sum, one more over the row for the gradient.
-template <class T, int THREADS, bool GRAD>
-__global__ __launch_bounds__(THREADS) void k_logits_density(const DensityArgs a) {
-  constexpr int N = kPer<T>;
+template <class C> M355_DEV C wave_max(C v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max_c(v, (C)__shfl_xor(v, o, 64));
+  return v;
+}
+template <class C> M355_DEV C wave_sum(C v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += (C)__shfl_xor(v, o, 64);
+  return v;
+}
+
+// The thread's piece of the j-th round of THREADS pieces: a uniform address plus a 32-bit offset that all rounds share
+template <class T, int THREADS> M355_DEV const raw_t<T>* piece(const typename T::store* row, int j) {
+  return reinterpret_cast<const raw_t<T>*>(reinterpret_cast<const char*>(row) + (size_t)j * (THREADS * 16) +
+                                           (unsigned)threadIdx.x * 16u);
+}
+template <class T, int THREADS> M355_DEV raw_t<T>* piece(typename T::store* row, int j) {
+  return reinterpret_cast<raw_t<T>*>(reinterpret_cast<char*>(row) + (size_t)j * (THREADS * 16) + (unsigned)threadIdx.x * 16u);
+}
+
+template <class T> M355_DEV raw_t<T> raw_lowest() {  // kPer times -inf
+  typename T::comp t[kPer<T>];
+#pragma unroll
+  for (int e = 0; e < kPer<T>; ++e) t[e] = (typename T::comp)-kInf;
+  return pack<T>(t);
+}
+
+// Keeps the compiler from carrying the unpacked elements of one pass over the registers into the next (twice the
+// registers for 16-bit types, which then spill): to it the pieces may have changed.  No instruction.
+template <class T> M355_DEV void repack(raw_t<T>& r) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  u4 v = {r.x, r.y, r.z, r.w};
+  asm volatile("" : "+v"(v));
+  r.x = v.x, r.y = v.y, r.z = v.z, r.w = v.w;
+}
+
+// Value and gradient, one row per workgroup.  The row is read once: its first NR * THREADS 16-byte pieces wait in registers,
+// the next NL * THREADS in LDS, while maximum and sum are formed; what does not fit there is summed as it passes and read
+// again for the gradient.  The k % kPer last elements belong to the first threads, one each.  In place (grad == z): a row is
+// read before it is written, but for the pieces that are read again, which the same thread reads and writes.
+template <class T, int THREADS, int NR, int NL, int WAVES, bool REST>
+__global__ __launch_bounds__(THREADS, WAVES) void k_logits_grad(const DensityArgs a) {
   typedef typename T::comp comp;
   typedef typename T::store store;
+  constexpr int N = kPer<T>;
+  constexpr int W = THREADS / 64;
+  constexpr bool kKeepExp = sizeof(comp) == sizeof(store);  // exp(z) has room where z was (16 bits would not hold it)
+  constexpr int U = 4;  // loads in flight per thread of what passes by
+  __shared__ comp red[2][W];
+  __shared__ uint4 kept[NL ? NL * THREADS : 1];
+  const int tid = threadIdx.x, nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
+  const raw_t<T> lowest = raw_lowest<T>();
+  auto load = [&](const store* z, int j, int count) {
+    return tid < count - j * THREADS ? __builtin_nontemporal_load(piece<T, THREADS>(z, j)) : lowest;
+  };
+  // the number of pieces anew for every pass: the comparisons with it are cheaper than 2 * NR scalar registers to keep them
+  auto fresh = [](int count) {
+    asm volatile("" : "+s"(count));
+    return count;
+  };
+  auto to_lds = [&](int l, raw_t<T> r) { kept[l * THREADS + tid] = uint4{r.x, r.y, r.z, r.w}; };
+  auto from_lds = [&](int l) {  // a thread reads what it wrote itself: no barrier
+    const uint4 u = kept[l * THREADS + tid];
+    raw_t<T> r;
+    r.x = u.x, r.y = u.y, r.z = u.z, r.w = u.w;
+    return r;
+  };
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const store* z = static_cast<const store*>(a.z) + row * a.z_ld;
-    const comp w = GRAD ? (comp)row_operand(a.weight, row) : (comp)1;
+    store* g = static_cast<store*>(a.grad) + row * a.grad_ld;
+    const comp w = (comp)row_operand(a.weight, row);
+    const long long xi = observed(a, row);
+    if (w == (comp)0 || xi < 0) {  // the gradient is 0 whatever the row holds: it is not read
+      raw_t<T> none;
+      none.x = none.y = none.z = none.w = 0;
+      for (int i = tid; i < nv; i += THREADS) __builtin_nontemporal_store(none, reinterpret_cast<raw_t<T>*>(g + (long long)i * N));
+      if (tid < tail) g[(long long)nv * N + tid] = (store)0;
+      if (tid == 0) static_cast<comp*>(a.lp)[row] = (comp)-kInf;  // left out of the total where the weight is 0
+      continue;
+    }
+    raw_t<T> raw[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) raw[j] = load(z, j, nv);
+    const comp zx = (comp)z[xi];
+    const comp last = tid < tail ? (comp)z[(long long)nv * N + tid] : (comp)-kInf;
+#pragma unroll U
+    for (int l = 0; l < NL; ++l) to_lds(l, load(z, NR + l, nv));
+    comp m = last, s = 0;
+    comp ms = (comp)-kInf;  // maximum of what passes by; s is its sum
+    for (int base = (NR + NL) * THREADS + tid; REST && base < nv; base += U * THREADS) {
+      raw_t<T> r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) r[u] = base + u * THREADS < nv ? load_raw<T>(z + (long long)(base + u * THREADS) * N) : lowest;
+      comp mt = ms;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        comp t[N];
+        unpack<T>(r[u], t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) mt = max_c(mt, t[e]);
+      }
+      const comp b = finite_max(mt);
+      s *= exp_neg(ms - b);
+      ms = mt;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        comp t[N];
+        repack<T>(r[u]);
+        unpack<T>(r[u], t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += exp_neg(t[e] - b);
+      }
+    }
+    m = max_c(m, ms);
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      comp t[N];
+      unpack<T>(raw[j], t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) m = max_c(m, t[e]);
+    }
+#pragma unroll 2
+    for (int l = 0; l < NL; ++l) {
+      comp t[N];
+      unpack<T>(from_lds(l), t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) m = max_c(m, t[e]);
+    }
+    m = wave_max(m);
+    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max_c(m, red[0][i]);
+    const comp b = finite_max(m);
+    s = REST ? s * exp_neg(ms - b) + exp_neg(last - b) : exp_neg(last - b);
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      comp t[N];
+      repack<T>(raw[j]);
+      unpack<T>(raw[j], t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        t[e] = exp_neg(t[e] - b);
+        s += t[e];
+      }
+      if constexpr (kKeepExp) raw[j] = pack<T>(t);
+    }
+#pragma unroll 2
+    for (int l = 0; l < NL; ++l) {
+      comp t[N];
+      unpack<T>(from_lds(l), t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += exp_neg(t[e] - b);
+    }
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[1][tid >> 6] = s;
+    __syncthreads();  // red[0] is written again only behind this barrier, red[1] behind the next row's first
+    s = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += red[1][i];
+    if (tid == 0) static_cast<comp*>(a.lp)[row] = density(zx, m, s, true);
+    const bool zero = s == (comp)0;  // all -inf: every exp(z) is 0
+    const comp q = zero ? (comp)0 : -w / s;
+    auto gradient = [&](raw_t<T> r) {
+      comp t[N];
+      unpack<T>(r, t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) t[e] = exp_neg(t[e] - b) * q;
+      return pack<T>(t);
+    };
+    auto times = [](raw_t<T> r, comp f) {
+      comp t[N];
+      unpack<T>(r, t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) t[e] *= f;
+      return pack<T>(t);
+    };
+    const int here = fresh(nv);
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      if constexpr (!kKeepExp) repack<T>(raw[j]);
+      if (tid < here - j * THREADS)
+        __builtin_nontemporal_store(kKeepExp ? times(raw[j], q) : gradient(raw[j]), piece<T, THREADS>(g, j));
+    }
+#pragma unroll 2
+    for (int l = 0; l < NL; ++l)
+      if (tid < here - (NR + l) * THREADS) __builtin_nontemporal_store(gradient(from_lds(l)), piece<T, THREADS>(g, NR + l));
+    for (int base = (NR + NL) * THREADS + tid; REST && base < nv; base += U * THREADS) {
+      raw_t<T> r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) r[u] = base + u * THREADS < nv ? load_raw<T>(z + (long long)(base + u * THREADS) * N) : lowest;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + u * THREADS < nv)
+          __builtin_nontemporal_store(gradient(r[u]), reinterpret_cast<raw_t<T>*>(g + (long long)(base + u * THREADS) * N));
+    }
+    if (tid < tail) g[(long long)nv * N + tid] = (store)(exp_neg(last - b) * q);
+    if (!zero) {  // the observation's own element, by the thread that wrote it: after that store
+      const long long vi = xi / N;
+      if (vi < nv ? (int)(vi % THREADS) == tid : (int)(xi - (long long)nv * N) == tid) g[xi] = (store)(exp_neg(zx - b) * q + w);
+    }
+  }
+}
+
+// Value only: one row per workgroup, tiles of NR 16-byte loads per thread with a running maximum and sum.
+template <class T, int THREADS, int NR>
+__global__ __launch_bounds__(THREADS) void k_logits_value(const DensityArgs a) {
+  constexpr int N = kPer<T>;
+  constexpr int W = THREADS / 64;
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  __shared__ comp red[2][W];
+  const int tid = threadIdx.x, nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
+  const raw_t<T> lowest = raw_lowest<T>();
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const store* z = static_cast<const store*>(a.z) + row * a.z_ld;
     const long long xi = observed(a, row);
     const comp zx = xi >= 0 ? (comp)z[xi] : (comp)0;
-    comp m = (comp)-kInf, s = 0;
-    if (!GRAD || w != (comp)0) {
-      for (long long v = (long long)threadIdx.x * N; v < a.k; v += THREADS * N) {
-        comp t[N];
-        unpack<T>(load_row<T>(z, v, a.k, (comp)-kInf), t);
-        accumulate<T>(t, m, s);
-      }
-      block_join<THREADS>(m, s);  // its barriers also separate the read of z[xi] from the writes of the gradient
-    }
-    if (threadIdx.x == 0) static_cast<comp*>(a.lp)[row] = density(zx, m, s, xi >= 0);
-    if constexpr (GRAD) {
-      store* g = static_cast<store*>(a.grad) + row * a.grad_ld;
-      const comp b = finite_max(m);
-      const bool zero = w == (comp)0 || xi < 0 || s == (comp)0;
-      const comp q = zero ? (comp)0 : -w / s;
-      for (long long v = (long long)threadIdx.x * N; v < a.k; v += THREADS * N) {
-        comp t[N];
-        if (zero) {
+    comp m = tid < tail ? (comp)z[(long long)nv * N + tid] : (comp)-kInf;
+    comp s = exp_neg(m - finite_max(m));
+    for (int base = 0; base < nv; base += NR * THREADS) {
+      raw_t<T> raw[NR];
 #pragma unroll
-          for (int e = 0; e < N; ++e) t[e] = 0;
-        } else {
-          unpack<T>(load_row<T>(z, v, a.k, (comp)-kInf), t);
+      for (int j = 0; j < NR; ++j) {
+        const int i = base + j * THREADS + tid;
+        raw[j] = i < nv ? load_raw_nt<T>(z + (long long)i * N) : lowest;
+      }
+      comp mt = m;
 #pragma unroll
-          for (int e = 0; e < N; ++e) t[e] = exp_neg(t[e] - b) * q + (v + e == xi ? w : (comp)0);
-        }
-        store_row<T>(g, v, a.k, t);
+      for (int j = 0; j < NR; ++j) {
+        comp t[N];
+        unpack<T>(raw[j], t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) mt = max_c(mt, t[e]);
+      }
+      const comp b = finite_max(mt);
+      s *= exp_neg(m - b);
+      m = mt;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        comp t[N];
+        repack<T>(raw[j]);
+        unpack<T>(raw[j], t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += exp_neg(t[e] - b);
       }
     }
+    comp mm = wave_max(m);
+    s = wave_sum(s * exp_neg(m - finite_max(mm)));
+    if ((tid & 63) == 0) {
+      red[0][tid >> 6] = mm;
+      red[1][tid >> 6] = s;
+    }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 1; i < W; ++i) join<comp>(mm, s, red[0][i], red[1][i]);
+      static_cast<comp*>(a.lp)[row] = density(zx, mm, s, xi >= 0);
+    }
+    __syncthreads();
   }
 }
 
@@ -348,9 +535,17 @@ __global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp,
                                                        C* __restrict__ total) {
   __shared__ double red[16];
   double acc = 0.0;
-  for (long long r = threadIdx.x; r < rows; r += 1024) {
-    const double w = row_operand(weight, r);
-    if (w != 0.0) acc += w * (double)lp[r];
+  for (long long base = threadIdx.x; base < rows; base += 4096) {
+    double w[4], v[4];  // four rows' loads together: the launch is all latency
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long r = base + j * 1024;
+      w[j] = r < rows ? row_operand(weight, r) : 0.0;
+      v[j] = r < rows ? (double)lp[r] : 0.0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (w[j] != 0.0) acc += w[j] * v[j];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_down(acc, o, 64);
@@ -395,9 +590,32 @@ template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, dou
                      a.k, rb, dbias, a.bias_dtype);
 }
 
+template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launch_grad(const DensityArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_logits_grad<T, THREADS, NR, NL, WAVES, REST>),
+                     dim3((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid)), dim3(THREADS), 0, s, a);
+}
+
+// Pieces per thread and threads per workgroup by the row's length.  Measured for bf16 (r + w, 5.1-5.7 TB/s; a copy reaches
+// 6.4): four pieces per thread beat eight of half the threads while a row fits 1024 threads (8192 x 32768: 194 against
+// 208 us), then two workgroups of 512 threads a CU beat one of 1024 (4096 x 131072: 415 against 437-450 us) although
+// they read half of the row twice, from the Infinity Cache; rows over 256 KiB take one workgroup a CU again (float32,
+// 1500 x 100003: 256 against 277 us), because the rows of 512 workgroups no longer fit that cache.
 template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStream_t s) {
-  const unsigned grid = (unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid);
-  hipLaunchKernelGGL((k_logits_density<T, 256, GRAD>), dim3(grid), dim3(256), 0, s, a);
+  const long long nv = a.k / kPer<T>;
+  if constexpr (GRAD) {
+    constexpr bool wide = sizeof(typename T::store) == 8;
+    if (nv <= 256 * 2) launch_grad<T, 256, 2, 0, 4, false>(a, s);
+    else if (nv <= 256 * 4) launch_grad<T, 256, 4, 0, wide ? 4 : 8, false>(a, s);
+    else if (nv <= 512 * 4) launch_grad<T, 512, 4, 0, 4, false>(a, s);
+    else if (nv <= 1024 * 4) launch_grad<T, 1024, 4, 0, wide ? 4 : 8, false>(a, s);
+    else if (nv <= 512 * 16 && !wide) launch_grad<T, 512, wide ? 8 : 16, 0, 4, false>(a, s);
+    else if (nv <= 512 * 32 && !wide) launch_grad<T, 512, wide ? 8 : 16, 0, 4, true>(a, s);
+    else launch_grad<T, 1024, wide ? 6 : 8, wide ? 6 : 4, 4, true>(a, s);
+  } else {
+    const dim3 grid((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid));
+    if (a.rows >= 1024 || nv <= 256 * 4) hipLaunchKernelGGL((k_logits_value<T, 256, 8>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_logits_value<T, 1024, 8>), grid, dim3(1024), 0, s, a);
+  }
 }
 
 template <class F> int by_dtype(int dtype, F f) {
@@ -437,6 +655,7 @@ int row_arg(const m355_operand& in, int64_t rows, m355::DevOperand& out, const c
   if (in.div < 1 || in.mod < 1) return fail(M355_ERR_INVALID, "%s: div and mod must be >= 1", what);
   out.div = (unsigned long long)in.div;
   out.mod = in.div >= rows ? 1 : (unsigned long long)in.mod;
+  if (out.div == 1 && out.mod >= (unsigned long long)rows) out.mod = 0;  // one value per row: no division per access
   return 0;
 }
 

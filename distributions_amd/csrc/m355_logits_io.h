@@ -92,10 +92,10 @@ M355_DEV void store_row(typename T::store* row, long long v, long long k, const 
     if (v + e < k) row[v + e] = (typename T::store)t[e];
 }
 
-// A per-row argument (scalar, or float64 / float32 array indexed by (row / div) % mod)
+// A per-row argument: scalar, or float64 / float32 array indexed by the row (mod == 0) or by (row / div) % mod
 M355_DEV double row_operand(const DevOperand& o, long long row) {
   if (!o.ptr) return o.scalar;
-  const unsigned long long i = o.mod == 1 ? 0 : ((unsigned long long)row / o.div) % o.mod;
+  const unsigned long long i = o.mod == 0 ? row : o.mod == 1 ? 0 : ((unsigned long long)row / o.div) % o.mod;
   return o.dtype == M355_F32 ? (double)static_cast<const float*>(o.ptr)[i] : static_cast<const double*>(o.ptr)[i];
 }
 
