@@ -30,188 +30,334 @@ struct AdjustArgs {
   long long mask_ld;
 };
 
-// kPer flags for the elements from v on (v is a multiple of kPer): bit e = element v + e is allowed
-template <class T> M355_DEV unsigned mask_flags(const AdjustArgs& a, long long row, long long v) {
-  constexpr int N = kPer<T>;
-  if (a.mask_kind == M355_MASK_NONE) return (1u << N) - 1;
-  if (a.mask_kind == M355_MASK_BITS) {
-    const unsigned w = static_cast<const unsigned*>(a.mask)[row * a.mask_ld + (v >> 5)];
-    return (w >> (v & 31)) & ((1u << N) - 1);
+// Whether category v is allowed
+M355_DEV bool allowed(const AdjustArgs& a, long long row, long long v) {
+  if (a.mask_kind == M355_MASK_NONE) return true;
+  if (a.mask_kind == M355_MASK_BITS) return (static_cast<const unsigned*>(a.mask)[row * a.mask_ld + (v >> 5)] >> (v & 31)) & 1;
+  return static_cast<const unsigned char*>(a.mask)[row * a.mask_ld + v] != 0;
+}
+// The mask of a whole piece (v is a multiple of kPer, v + kPer <= k): the raw bytes resp. the word, then its kPer flags
+template <class T> struct MaskPiece {
+  unsigned long long bytes;
+  M355_DEV void load(const AdjustArgs& a, long long row, long long v) {
+    bytes = ~0ull;
+    if (a.mask_kind == M355_MASK_BYTES)
+      __builtin_memcpy(&bytes, static_cast<const unsigned char*>(a.mask) + row * a.mask_ld + v, kPer<T>);
+    else if (a.mask_kind == M355_MASK_BITS)
+      bytes = static_cast<const unsigned*>(a.mask)[row * a.mask_ld + (v >> 5)] >> (v & 31);
   }
-  const unsigned char* m = static_cast<const unsigned char*>(a.mask) + row * a.mask_ld + v;
-  unsigned f = 0;
-  if (v + N <= a.k) {
-    unsigned char b[N];
-    __builtin_memcpy(b, m, N);
+  M355_DEV bool operator()(const AdjustArgs& a, int e) const {
+    return a.mask_kind == M355_MASK_BYTES ? ((bytes >> (8 * e)) & 0xff) != 0 : ((bytes >> e) & 1) != 0;
+  }
+};
+
+// kPer values of the bias, of type B: the logits' own, or float32 next to 16-bit logits (two loads)
+template <class T, class B> struct BiasPiece {
+  static constexpr int kLoads = kPer<T> / kPer<B>;
+  raw_t<B> raw[kLoads];
+  M355_DEV void load(const AdjustArgs& a, long long row, long long v) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) f |= (b[e] != 0 ? 1u : 0u) << e;
+    for (int h = 0; h < kLoads; ++h)
+      raw[h] = load_raw<B>(static_cast<const typename B::store*>(a.bias) + row * a.bias_ld + v + h * kPer<B>);
+  }
+  M355_DEV void add_to(typename T::comp (&s)[kPer<T>]) const {
+#pragma unroll
+    for (int h = 0; h < kLoads; ++h) {
+      typename B::comp b[kPer<B>];
+      unpack<B>(raw[h], b);
+#pragma unroll
+      for (int e = 0; e < kPer<B>; ++e) s[h * kPer<B> + e] += b[e];
+    }
+  }
+};
+template <class T> struct BiasPiece<T, void> {
+  M355_DEV void load(const AdjustArgs&, long long, long long) {}
+  M355_DEV void add_to(typename T::comp (&)[kPer<T>]) const {}
+};
+
+// 1 / temperature of a row: one rounding more than a division per element, which would cost more than the rest of the body
+template <class C> M355_DEV C inverse_temperature(const AdjustArgs& a, long long row) { return (C)1 / (C)row_operand(a.temp, row); }
+
+struct AdjustGrid {
+  long long items;
+  int chunks, per;    // a row is cut into `chunks` of `per` pieces (of kPer categories)
+  bool rows_by_xcd;  // see item_of
+};
+// (row, chunk) of a work item.  Workgroups are dealt to the eight XCDs in turn; with many rows all chunks of a row go to one
+// of them, so that the row's history and mask words are fetched into one L2 and not into eight.
+M355_DEV bool item_of(const AdjustArgs& a, const AdjustGrid& g, long long item, long long& row, int& chunk) {
+  if (g.rows_by_xcd) {
+    const long long local = item >> 3;
+    row = local / g.chunks * 8 + (item & 7);
+    chunk = (int)(local % g.chunks);
   } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (v + e < a.k) f |= (m[e] != 0 ? 1u : 0u) << e;
+    row = item / g.chunks;
+    chunk = (int)(item % g.chunks);
   }
-  return f;
+  return row < a.rows;
 }
 
-template <class T> M355_DEV void load_bias(const AdjustArgs& a, long long row, long long v, typename T::comp (&b)[kPer<T>]) {
-  if (a.bias_dtype == T::kCode) {
-    unpack<T>(load_row<T>(static_cast<const typename T::store*>(a.bias) + row * a.bias_ld, v, a.k, 0), b);
-  } else {  // float32 next to 16-bit logits
-    const float* p = static_cast<const float*>(a.bias) + row * a.bias_ld;
+// Occurrences of the categories [base, base + width) in the row's history, in LDS: twice the number among the generated ids,
+// plus 1 if the prompt has it, in C-sized counters: 32 bits, or 16 where the history is short enough for them.  One
+// atomic per id; additions of integers: their order does not matter.
+template <class C> M355_DEV void count_one(unsigned* counts, unsigned at, bool generated) {
+  if (sizeof(C) == 2) {
+    if (generated) atomicAdd(&counts[at >> 1], 2u << (16 * (at & 1)));
+    else atomicOr(&counts[at >> 1], 1u << (16 * (at & 1)));
+  } else {
+    if (generated) atomicAdd(&counts[at], 2u);
+    else atomicOr(&counts[at], 1u);
+  }
+}
+template <class C, class ID, int THREADS>
+M355_DEV void count_history(const AdjustArgs& a, long long row, long long base, unsigned width, unsigned* counts) {
+  constexpr int U = 8;  // ids in flight per thread: the loop is all latency
+  const ID* h = static_cast<const ID*>(a.history) + row * a.history_ld;
+  // the first ids are fetched before the row's length is known; those behind it are dropped
+  ID id[U];
 #pragma unroll
-    for (int h = 0; h < kPer<T>; h += 4) {
-      float t[4];
-      unpack<F32>(load_row<F32>(p, v + h < a.k ? v + h : 0, v + h < a.k ? a.k : 0, 0.0f), t);
+  for (int u = 0; u < U; ++u) {
+    const int i = u * THREADS + (int)threadIdx.x;
+    id[u] = i < a.history_len ? h[i] : (ID)-1;
+  }
+  long long len = a.lengths ? a.lengths[row] : a.history_len;
+  len = len < 0 ? 0 : (len > a.history_len ? a.history_len : len);
+  const long long prompt = a.prompts ? a.prompts[row] : 0;
+  for (int first = 0;;) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (h + e < kPer<T>) b[h + e] = (typename T::comp)t[e];
+    for (int u = 0; u < U; ++u) {
+      const int i = first + u * THREADS + (int)threadIdx.x;
+      const unsigned long long at = (unsigned long long)((long long)id[u] - base);
+      if (i < len && at < width) count_one<C>(counts, (unsigned)at, i >= prompt);
+    }
+    if (first >= len - U * THREADS) break;
+    first += U * THREADS;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = (long long)first + u * THREADS + (int)threadIdx.x;
+      id[u] = i < len ? h[i] : (ID)-1;
     }
   }
 }
 
-constexpr int kAdjThreads = 256;
+template <class C> M355_DEV C penalised(C s, unsigned count, C rep, C pres, C freq) {
+  if (count) s = s > 0 ? s / rep : s * rep;
+  if (count >> 1) s -= freq * (C)(count >> 1) + pres;
+  return s;
+}
 
-// One workgroup per (row, chunk of kAdjThreads * VPT * kPer categories).  With a history the workgroup first counts the
-// ids that fall into its chunk in LDS (word = 2 * generated + [in the prompt]: one atomic per id), then streams its chunk.
-template <class T, int VPT, bool HIST, bool BWD>
-__global__ __launch_bounds__(kAdjThreads) void k_logits_adjust(const AdjustArgs a, long long items, int chunks) {
-  constexpr int N = kPer<T>;
-  constexpr int C = kAdjThreads * VPT * N;
+// One workgroup per (row, chunk): everything the chunk needs from memory is fetched first, then, with a history (CNT: the
+// type of its counters, or void), the ids that fall into the chunk are counted in LDS, then the pieces are worked off.  The
+// k % kPer last categories of a row belong to the first threads of its last chunk.
+template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD>
+__global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustArgs a, const AdjustGrid grid) {
   typedef typename T::comp comp;
   typedef typename T::store store;
-  extern __shared__ unsigned counts[];  // C words with HIST
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const long long row = item / chunks;
-    const long long base = (item - row * chunks) * C;
+  constexpr int N = kPer<T>;
+  constexpr bool HIST = !std::is_void<CNT>::value;
+  typedef typename std::conditional<HIST, CNT, unsigned>::type cnt;
+  constexpr int kCounts = HIST ? (THREADS * VPT + 1) * N : 4;  // one piece more for the tail
+  __shared__ uint4 count_store[(kCounts * sizeof(cnt) + 15) / 16];
+  cnt* counts = reinterpret_cast<cnt*>(count_store);
+  const int tid = threadIdx.x, nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
+  for (long long item = blockIdx.x; item < grid.items; item += gridDim.x) {
+    long long row;
+    int chunk;
+    if (!item_of(a, grid, item, row, chunk)) continue;
+    const int c0 = chunk * grid.per, c1 = c0 + grid.per < nv ? c0 + grid.per : nv;  // pieces of the chunk
+    const long long base = (long long)c0 * N;
+    const bool has_tail = chunk == grid.chunks - 1 && tid < tail;
+    const long long vt = (long long)nv * N + tid;
     const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
     raw_t<T> raw[VPT];
+    MaskPiece<T> mask[VPT];
+    BiasPiece<T, typename std::conditional<BWD, void, B>::type> bias[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const long long v = base + (j * kAdjThreads + threadIdx.x) * N;
-      if (v < a.k) raw[j] = load_row<T>(src, v, a.k, 0);
+      const int i = c0 + j * THREADS + tid;
+      if (i >= c1) continue;
+      const long long v = (long long)i * N;
+      raw[j] = load_raw<T>(src + v);
+      mask[j].load(a, row, v);
+      bias[j].load(a, row, v);
     }
     comp rep = 1, pres = 0, freq = 0;
     if constexpr (HIST) {
-#pragma unroll
-      for (int j = 0; j < VPT * N / 4; ++j)
-        reinterpret_cast<uint4*>(counts)[j * kAdjThreads + threadIdx.x] = uint4{0, 0, 0, 0};
+      for (int i = tid; i < (int)(sizeof(count_store) / 16); i += THREADS) count_store[i] = uint4{0, 0, 0, 0};
       __syncthreads();
       const long long left = a.k - base;
-      const unsigned long long width = left < C ? left : C;
-      long long len = a.lengths ? a.lengths[row] : a.history_len;
-      len = len < 0 ? 0 : (len > a.history_len ? a.history_len : len);
-      const long long prompt = a.prompts ? a.prompts[row] : 0;
-      for (int i = threadIdx.x; i < (int)len; i += kAdjThreads) {
-        const long long id = a.history_dtype == M355_I64
-                                 ? static_cast<const long long*>(a.history)[row * a.history_ld + i]
-                                 : (long long)static_cast<const int*>(a.history)[row * a.history_ld + i];
-        const unsigned long long at = (unsigned long long)(id - base);
-        if (id >= 0 && at < width) {
-          if (i >= prompt) atomicAdd(&counts[at], 2u);
-          else atomicOr(&counts[at], 1u);
-        }
-      }
+      const unsigned width = chunk == grid.chunks - 1 ? (unsigned)left : (unsigned)((c1 - c0) * N);
+      if (a.history_dtype == M355_I64) count_history<cnt, long long, THREADS>(a, row, base, width, reinterpret_cast<unsigned*>(counts));
+      else count_history<cnt, int, THREADS>(a, row, base, width, reinterpret_cast<unsigned*>(counts));
       __syncthreads();
       rep = (comp)row_operand(a.rep, row);
       pres = (comp)row_operand(a.pres, row);
       freq = (comp)row_operand(a.freq, row);
     }
-    // one rounding more than a division per element, which would cost more than the rest of the body
-    const comp inv_t = (comp)(1.0 / row_operand(a.temp, row));
+    const comp inv_t = inverse_temperature<comp>(a, row);
+    store* dst = static_cast<store*>(a.dst) + row * a.dst_ld;
+    const store* x = static_cast<const store*>(a.x) + row * a.x_ld;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int at = (j * kAdjThreads + threadIdx.x) * N;
-      const long long v = base + at;
-      if (v >= a.k) continue;
+      const int i = c0 + j * THREADS + tid;
+      if (i >= c1) continue;
+      const long long v = (long long)i * N;
       comp s[N];
       unpack<T>(raw[j], s);
-      const unsigned ok = mask_flags<T>(a, row, v);
+      cnt count[N];
+      bool any = false;  // most pieces have no id of the history
+      if constexpr (HIST) {
+        __builtin_memcpy(count, counts + (i - c0) * N, sizeof(count));
+#pragma unroll
+        for (int e = 0; e < N; ++e) any |= count[e] != 0;
+      }
       if constexpr (!BWD) {
-        if constexpr (HIST) {
+        if (any) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const unsigned c = counts[at + e];
-            if (c) {
-              s[e] = s[e] > 0 ? s[e] / rep : s[e] * rep;
-              if (c >> 1) s[e] -= freq * (comp)(c >> 1) + pres;
-            }
-          }
+          for (int e = 0; e < N; ++e) s[e] = penalised<comp>(s[e], count[e], rep, pres, freq);
         }
-        if (a.bias) {
-          comp b[N];
-          load_bias<T>(a, row, v, b);
+        bias[j].add_to(s);
 #pragma unroll
-          for (int e = 0; e < N; ++e) s[e] += b[e];
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)-kInf;
-        store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+        for (int e = 0; e < N; ++e) s[e] = mask[j](a, e) ? s[e] * inv_t : (comp)-kInf;
+        __builtin_nontemporal_store(pack<T>(s), reinterpret_cast<raw_t<T>*>(dst + v));
       } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)0;
-        if (a.dbias) {
-          if (a.bias_dtype == T::kCode) {
-            store_row<T>(static_cast<store*>(a.dbias) + row * a.k, v, a.k, s);
-          } else {
+        for (int e = 0; e < N; ++e) s[e] = mask[j](a, e) ? s[e] * inv_t : (comp)0;
+        if constexpr (!std::is_void<B>::value) {  // every row has its own bias: the gradient goes out as it is
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (v + e < a.k) static_cast<float*>(a.dbias)[row * a.k + v + e] = (float)s[e];
+          for (int h = 0; h < N; h += kPer<B>) {
+            typename B::comp t[kPer<B>];
+#pragma unroll
+            for (int e = 0; e < kPer<B>; ++e) t[e] = (typename B::comp)s[h + e];
+            store_raw_nt<B>(static_cast<typename B::store*>(a.dbias) + row * a.k + v + h, pack<B>(t));
           }
         }
-        if (!a.dst) continue;
-        if constexpr (HIST) {
-          const store* x = static_cast<const store*>(a.x) + row * a.x_ld;
+        if (a.dst) {
+          if (any) {
 #pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (counts[at + e]) s[e] = (comp)x[v + e] > 0 ? s[e] / rep : s[e] * rep;
+            for (int e = 0; e < N; ++e)
+              if (count[e]) s[e] = (comp)x[v + e] > 0 ? s[e] / rep : s[e] * rep;
+          }
+          store_raw_nt<T>(dst + v, pack<T>(s));
         }
-        store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+      }
+    }
+    if (has_tail) {
+      const unsigned count = HIST ? counts[vt - base] : 0;
+      comp s = (comp)src[vt];
+      const bool ok = allowed(a, row, vt);
+      if constexpr (!BWD) {
+        s = penalised<comp>(s, count, rep, pres, freq);
+        if constexpr (!std::is_void<B>::value) s += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + vt];
+        dst[vt] = (store)(ok ? s * inv_t : (comp)-kInf);
+      } else {
+        s = ok ? s * inv_t : (comp)0;
+        if constexpr (!std::is_void<B>::value)
+          static_cast<typename B::store*>(a.dbias)[row * a.k + vt] = (typename B::store)s;
+        if (a.dst) {
+          if (count) s = (comp)x[vt] > 0 ? s / rep : s * rep;
+          dst[vt] = (store)s;
+        }
       }
     }
     if constexpr (HIST) __syncthreads();  // the next item clears the counts
   }
 }
 
-// Gradient of a bias that all rows share: a thread owns kPer columns and walks a block of rows, so that the column sums
-// stay in its registers (float64); the partial sums of the row blocks are added in order by k_logits_cols_final.
-// Without a history the gradient of the logits is written on the way.
+// Gradient of a bias that all rows share.  A workgroup of kSumGroups x kSumThreads threads takes kSumThreads * kPer columns
+// and a block of rows; a thread owns kPer columns and every kSumGroups-th row of the block, so that the column sums stay in
+// its registers (float64) and kSumRows rows are in flight; the groups are joined in LDS, the row blocks by
+// k_logits_cols_final, all in a fixed order.  Without a history the gradient of the logits is written on the way.
+constexpr int kSumThreads = 128, kSumGroups = 4, kSumRows = 4;
+
 template <class T, bool WRITE>
-__global__ __launch_bounds__(kAdjThreads) void k_logits_adjust_cols(const AdjustArgs a, int chunks, int row_blocks,
-                                                                    double* __restrict__ partials) {
+__global__ __launch_bounds__(kSumThreads * kSumGroups) void k_logits_adjust_cols(const AdjustArgs a, int chunks,
+                                                                                 int row_blocks, double* __restrict__ partials) {
   constexpr int N = kPer<T>;
   typedef typename T::comp comp;
   typedef typename T::store store;
+  __shared__ double joined[kSumGroups - 1][N][kSumThreads];
+  const int col = threadIdx.x % kSumThreads, group = threadIdx.x / kSumThreads;
+  const int nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
   const int chunk = blockIdx.x % chunks, rb = blockIdx.x / chunks;
-  const long long v = ((long long)chunk * kAdjThreads + threadIdx.x) * N;
-  if (v >= a.k) return;
+  const int i = chunk * kSumThreads + col;  // the piece, or (from nv on) a single category of the tail
   const long long lo = a.rows * rb / row_blocks, hi = a.rows * (rb + 1) / row_blocks;
   double acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.0;
-  for (long long row = lo; row < hi; ++row) {
-    comp s[N];
-    unpack<T>(load_row<T>(static_cast<const store*>(a.src) + row * a.src_ld, v, a.k, 0), s);
-    const unsigned ok = mask_flags<T>(a, row, v);
-    const comp inv_t = (comp)(1.0 / row_operand(a.temp, row));
+  if (i < nv) {
+    const long long v = (long long)i * N;
+    for (long long first = lo + group; first < hi; first += kSumGroups * kSumRows) {
+      raw_t<T> raw[kSumRows];
+      MaskPiece<T> mask[kSumRows];
+      comp inv_t[kSumRows];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      s[e] = (ok >> e) & 1 ? s[e] * inv_t : (comp)0;
-      acc[e] += (double)s[e];
+      for (int r = 0; r < kSumRows; ++r) {
+        const long long row = first + r * kSumGroups;
+        if (row >= hi) continue;
+        raw[r] = __builtin_nontemporal_load(reinterpret_cast<const raw_t<T>*>(static_cast<const store*>(a.src) + row * a.src_ld + v));
+        mask[r].load(a, row, v);
+        inv_t[r] = inverse_temperature<comp>(a, row);
+      }
+#pragma unroll
+      for (int r = 0; r < kSumRows; ++r) {
+        const long long row = first + r * kSumGroups;
+        if (row >= hi) continue;
+        comp s[N];
+        unpack<T>(raw[r], s);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          s[e] = mask[r](a, e) ? s[e] * inv_t[r] : (comp)0;
+          acc[e] += (double)s[e];
+        }
+        if constexpr (WRITE) store_raw_nt<T>(static_cast<store*>(a.dst) + row * a.dst_ld + v, pack<T>(s));
+      }
     }
-    if constexpr (WRITE) store_row<T>(static_cast<store*>(a.dst) + row * a.dst_ld, v, a.k, s);
+  } else if (i - nv < tail) {
+    const long long v = (long long)nv * N + (i - nv);
+    for (long long row = lo + group; row < hi; row += kSumGroups) {
+      const comp s = allowed(a, row, v) ? (comp) static_cast<const store*>(a.src)[row * a.src_ld + v] * inverse_temperature<comp>(a, row)
+                                        : (comp)0;
+      acc[0] += (double)s;
+      if constexpr (WRITE) static_cast<store*>(a.dst)[row * a.dst_ld + v] = (store)s;
+    }
   }
+  if (group > 0) {
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (v + e < a.k) partials[(long long)rb * a.k + v + e] = acc[e];
+    for (int e = 0; e < N; ++e) joined[group - 1][e][col] = acc[e];
+  }
+  __syncthreads();
+  if (group == 0) {
+#pragma unroll
+    for (int g = 0; g < kSumGroups - 1; ++g)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += joined[g][e][col];
+    double* out = partials + (long long)rb * a.k;
+    if (i < nv) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[(long long)i * N + e] = acc[e];
+    } else if (i - nv < tail) {
+      out[(long long)nv * N + (i - nv)] = acc[0];
+    }
+  }
 }
 
+// Sums the row blocks: 64 columns by 4 groups of row blocks a workgroup, joined in order
 template <class T>
-__global__ __launch_bounds__(kAdjThreads) void k_logits_cols_final(const double* __restrict__ partials, long long k,
-                                                                   int row_blocks, void* __restrict__ out, int odt) {
-  const long long v = (long long)blockIdx.x * kAdjThreads + threadIdx.x;
-  if (v >= k) return;
+__global__ __launch_bounds__(256) void k_logits_cols_final(const double* __restrict__ partials, long long k, int row_blocks,
+                                                           void* __restrict__ out, int odt) {
+  __shared__ double joined[4][64];
+  const int col = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const long long v = (long long)blockIdx.x * 64 + col;
   double s = 0.0;
-  for (int b = 0; b < row_blocks; ++b) s += partials[(long long)b * k + v];
+  if (v < k) {
+#pragma unroll 4
+    for (int b = group; b < row_blocks; b += 4) s += partials[(long long)b * k + v];
+  }
+  joined[group][col] = s;
+  __syncthreads();
+  if (group != 0 || v >= k) return;
+  s = ((joined[0][col] + joined[1][col]) + joined[2][col]) + joined[3][col];
   if (odt == T::kCode) static_cast<typename T::store*>(out)[v] = (typename T::store)s;
   else static_cast<float*>(out)[v] = (float)s;
 }
@@ -560,34 +706,54 @@ __global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp,
 // ---------------------------------------------------------------------------------------------- launches
 constexpr long long kMaxGrid = 1ll << 30;
 
-template <class T, int VPT, bool HIST, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
-  constexpr int C = kAdjThreads * VPT * kPer<T>;
-  const long long chunks = (a.k + C - 1) / C, items = a.rows * chunks;
-  hipLaunchKernelGGL((k_logits_adjust<T, VPT, HIST, BWD>), dim3((unsigned)(items < kMaxGrid ? items : kMaxGrid)),
-                     dim3(kAdjThreads), HIST ? C * sizeof(unsigned) : 0, s, a, items, (int)chunks);
+template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+  const long long nv = a.k / kPer<T>;
+  AdjustGrid g;
+  g.chunks = (int)((nv + THREADS * VPT - 1) / (THREADS * VPT));
+  if (g.chunks < 1) g.chunks = 1;
+  g.per = (int)((nv + g.chunks - 1) / g.chunks);  // chunks of one size
+  if (g.per > 0) g.chunks = (int)((nv + g.per - 1) / g.per);  // and none that is empty
+  g.rows_by_xcd = a.rows >= 64;
+  g.items = (g.rows_by_xcd ? (a.rows + 7) / 8 * 8 : a.rows) * g.chunks;
+  hipLaunchKernelGGL((k_logits_adjust<T, THREADS, VPT, WAVES, CNT, B, BWD>), dim3((unsigned)(g.items < kMaxGrid ? g.items : kMaxGrid)),
+                     dim3(THREADS), 0, s, a, g);
 }
 
+template <class T, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+  // Four pieces per thread hide the latencies of a chunk behind each other; where that gives too few workgroups for 256
+  // CUs, one piece each (1 x 32768 bf16: 4.9 against 7.1 us).  512 threads halve how often a history is scanned, and cost
+  // more than they save (512 x 131072 bf16, 500 ids: 71 against 60 us; 256 x 65536, 8000 ids: 36.8 against 37.6 us).
+  const bool few = a.rows * (a.k / kPer<T>) < 256ll * 1024;
+  if (!a.history) few ? launch_adjust<T, 256, 1, 8, void, B, BWD>(a, s) : launch_adjust<T, 256, 4, 4, void, B, BWD>(a, s);
+  else if (a.history_len > 32767) launch_adjust<T, 256, 4, 4, unsigned, B, BWD>(a, s);
+  else if (few) launch_adjust<T, 256, 1, 8, unsigned short, B, BWD>(a, s);
+  else launch_adjust<T, 256, 4, 4, unsigned short, B, BWD>(a, s);
+}
+
+// forward: with the bias, if there is one; gradient: with a bias' gradient that goes out per element
 template <class T, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
-  if (a.history) launch_adjust<T, 4, true, BWD>(a, s);
-  else launch_adjust<T, 4, false, BWD>(a, s);
+  if (!(BWD ? a.dbias : a.bias)) launch_adjust<T, void, BWD>(a, s);
+  else if (a.bias_dtype == T::kCode) launch_adjust<T, T, BWD>(a, s);
+  else if constexpr (kPer<T> == 8) launch_adjust<T, F32, BWD>(a, s);
 }
 
-// row blocks of k_logits_adjust_cols: enough workgroups to fill the chip, at least eight rows each
+// column chunks and row blocks of k_logits_adjust_cols: about two workgroups per CU, at least kSumGroups * kSumRows rows each
+template <class T> int col_chunks_of(long long k) {
+  return (int)((k / kPer<T> + k % kPer<T> + kSumThreads - 1) / kSumThreads);
+}
 template <class T> int row_blocks_of(long long rows, long long k) {
-  const long long chunks = (k + kAdjThreads * kPer<T> - 1) / (kAdjThreads * kPer<T>);
-  long long rb = 2048 / chunks;
-  if (rb > rows / 8) rb = rows / 8;
+  long long rb = 1024 / col_chunks_of<T>(k);
+  if (rb > rows / (kSumGroups * kSumRows)) rb = rows / (kSumGroups * kSumRows);
   return (int)(rb < 1 ? 1 : rb);
 }
 
 template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, double* ws, hipStream_t s) {
-  const int chunks = (int)((a.k + kAdjThreads * kPer<T> - 1) / (kAdjThreads * kPer<T>));
-  const int rb = row_blocks_of<T>(a.rows, a.k);
-  const dim3 grid((unsigned)((long long)chunks * rb)), block(kAdjThreads);
+  const int chunks = col_chunks_of<T>(a.k), rb = row_blocks_of<T>(a.rows, a.k);
+  const dim3 grid((unsigned)((long long)chunks * rb)), block(kSumThreads * kSumGroups);
   if (a.dst) hipLaunchKernelGGL((k_logits_adjust_cols<T, true>), grid, block, 0, s, a, chunks, rb, ws);
   else hipLaunchKernelGGL((k_logits_adjust_cols<T, false>), grid, block, 0, s, a, chunks, rb, ws);
-  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + kAdjThreads - 1) / kAdjThreads)), block, 0, s, ws,
-                     a.k, rb, dbias, a.bias_dtype);
+  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + 63) / 64)), dim3(256), 0, s, ws, a.k, rb, dbias,
+                     a.bias_dtype);
 }
 
 template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launch_grad(const DensityArgs& a, hipStream_t s) {
