@@ -1,8 +1,8 @@
 // 2-norm over a list of tensors and clipping by it (include/m355_dist.h).  The list travels in the kernel arguments, up
-// to kListMax tensors a launch: nothing is uploaded, nothing is kept between calls, and a captured graph holds its own
-// copy.  The tensors of a launch are cut into chunks of kChunkVecs 16-byte accesses per thread that never cross a tensor;
-// workgroups take chunks in turn.  Squares are added in float64 (a float32 square overflows at 1.8e19, and the float64
-// fused multiply-adds cost a tenth of the memory time); one partial sum per workgroup, added in a fixed order.
+// to kListMax tensors of one type a launch: nothing is uploaded, nothing is kept between calls, and a captured graph holds
+// its own copy.  The tensors of a launch are cut into chunks of kChunkVecs 16-byte accesses per thread that never cross a
+// tensor.  Squares are added in float64 (a float32 square overflows at 1.8e19, and the float64 multiply-adds cost a fifth of
+// the memory time); one partial sum per workgroup, added in a fixed order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -16,8 +16,9 @@ namespace m355 {
 
 constexpr int kListMax = 128;     // 3712 bytes of kernel arguments
 constexpr int kListThreads = 256;
-constexpr int kChunkVecs = 8;     // 16-byte accesses in flight per thread
+constexpr int kChunkVecs = 4;     // 16-byte accesses in flight per thread
 constexpr int kNormBlocks = 2048;  // workgroups per launch of the norm: partial sums
+constexpr int kFinalThreads = 1024;
 
 struct TensorList {
   int count, chunks;
@@ -25,11 +26,11 @@ struct TensorList {
   void* out[kListMax];
   long long n[kListMax];
   int first[kListMax];  // index of the tensor's first chunk
-  unsigned char dtype[kListMax];
 };
 
 template <class T> constexpr long long kChunkElems = (long long)kListThreads * kChunkVecs * kPer<T>;
 
+// the tensor a chunk belongs to: the last one that begins at or before it (scalar loads of kernel arguments)
 M355_DEV int tensor_of(const TensorList& l, int chunk) {
   int lo = 0, hi = l.count - 1;
   while (lo < hi) {
@@ -39,71 +40,77 @@ M355_DEV int tensor_of(const TensorList& l, int chunk) {
   return lo;
 }
 
-template <class T> M355_DEV double sum_squares(const void* in, long long n, long long base) {
-  const typename T::store* p = static_cast<const typename T::store*>(in);
-  constexpr int N = kPer<T>;
-  raw_t<T> raw[kChunkVecs];
-#pragma unroll
-  for (int j = 0; j < kChunkVecs; ++j) {
-    const long long v = base + (j * kListThreads + (int)threadIdx.x) * N;
-    if (v < n) raw[j] = load_row<T>(p, v, n, 0);
+// A thread's pieces of a chunk: full 16-byte accesses, and the tensor's last n % kPer elements singly by the first threads of
+// its last chunk.
+template <class T> struct Chunk {
+  const typename T::store* p;
+  long long at, left;  // element of the thread's first piece; elements of the tensor from there on
+  M355_DEV Chunk(const TensorList& l, int t, int c)
+      : p(static_cast<const typename T::store*>(l.in[t])),
+        at((c - l.first[t]) * kChunkElems<T> + (int)threadIdx.x * kPer<T>),
+        left(l.n[t] - at) {}
+  M355_DEV bool whole(int j) const { return left >= ((long long)j * kListThreads + 1) * kPer<T>; }
+  // the element of the tensor's tail that is this thread's, or -1
+  M355_DEV long long tail(const TensorList& l, int t, int c) const {
+    const long long n = l.n[t], full = n / kPer<T> * kPer<T>;
+    const bool last = (c - l.first[t] + 1) * kChunkElems<T> >= n;
+    return last && full + (int)threadIdx.x < n ? full + (int)threadIdx.x : -1;
   }
-  double acc = 0.0;
-#pragma unroll
-  for (int j = 0; j < kChunkVecs; ++j) {
-    const long long v = base + (j * kListThreads + (int)threadIdx.x) * N;
-    if (v >= n) continue;
-    typename T::comp t[N];
-    unpack<T>(raw[j], t);
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc = __builtin_fma((double)t[e], (double)t[e], acc);
-  }
-  return acc;
-}
+};
 
-template <class T> M355_DEV void scale_chunk(const void* in, void* out, long long n, long long base, double f) {
-  const typename T::store* p = static_cast<const typename T::store*>(in);
+// A workgroup takes a run of neighbouring chunks: the tensor is searched once and then followed, and the next chunk's loads
+// are under way while this one's squares are added.
+template <class T> __global__ __launch_bounds__(kListThreads) void k_norm_partials(const TensorList l, double* __restrict__ partials) {
   constexpr int N = kPer<T>;
-  raw_t<T> raw[kChunkVecs];
+  const int lo = (int)((long long)l.chunks * blockIdx.x / gridDim.x), hi = (int)((long long)l.chunks * (blockIdx.x + 1) / gridDim.x);
+  raw_t<T> none;
+  none.x = none.y = none.z = none.w = 0;
+  raw_t<T> raw[2][kChunkVecs];
+  double acc[2] = {0.0, 0.0};
+  int t = tensor_of(l, lo);
+  auto fetch = [&](int c, raw_t<T>(&r)[kChunkVecs]) {
+    while (t + 1 < l.count && l.first[t + 1] <= c) ++t;
+    const Chunk<T> k(l, t, c);
 #pragma unroll
-  for (int j = 0; j < kChunkVecs; ++j) {
-    const long long v = base + (j * kListThreads + (int)threadIdx.x) * N;
-    if (v < n) raw[j] = load_row<T>(p, v, n, 0);
-  }
-#pragma unroll
-  for (int j = 0; j < kChunkVecs; ++j) {
-    const long long v = base + (j * kListThreads + (int)threadIdx.x) * N;
-    if (v >= n) continue;
-    typename T::comp t[N];
-    unpack<T>(raw[j], t);
-    // the product in float64, rounded to float32 on the way to a 16-bit type (twice rounded: off by at most 2^-25 more)
-#pragma unroll
-    for (int e = 0; e < N; ++e) t[e] = (typename T::comp)((double)t[e] * f);
-    store_row<T>(static_cast<typename T::store*>(out), v, n, t);
-  }
-}
-
-__global__ __launch_bounds__(kListThreads) void k_norm_partials(const TensorList l, double* __restrict__ partials) {
-  double acc = 0.0;
-  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
-    const int t = tensor_of(l, c);
-    const long long i = c - l.first[t];
-    switch (l.dtype[t]) {
-      case M355_F64: acc += sum_squares<F64>(l.in[t], l.n[t], i * kChunkElems<F64>); break;
-      case M355_F32: acc += sum_squares<F32>(l.in[t], l.n[t], i * kChunkElems<F32>); break;
-      case M355_F16: acc += sum_squares<F16>(l.in[t], l.n[t], i * kChunkElems<F16>); break;
-      default: acc += sum_squares<BF16>(l.in[t], l.n[t], i * kChunkElems<BF16>); break;
+    for (int j = 0; j < kChunkVecs; ++j) r[j] = k.whole(j) ? load_raw<T>(k.p + k.at + (long long)j * kListThreads * N) : none;
+    const long long e = k.tail(l, t, c);
+    if (e >= 0) {
+      const double v = (double)k.p[e];
+      acc[0] = __builtin_fma(v, v, acc[0]);
     }
+  };
+  auto add = [&](const raw_t<T>(&r)[kChunkVecs]) {
+#pragma unroll
+    for (int j = 0; j < kChunkVecs; ++j) {
+      typename T::comp v[N];
+      unpack<T>(r[j], v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e & 1] = __builtin_fma((double)v[e], (double)v[e], acc[e & 1]);
+    }
+  };
+  if (lo < hi) fetch(lo, raw[0]);
+  for (int c = lo; c < hi; c += 2) {
+    if (c + 1 < hi) fetch(c + 1, raw[1]);
+    add(raw[0]);
+    if (c + 1 >= hi) break;
+    if (c + 2 < hi) fetch(c + 2, raw[0]);
+    add(raw[1]);
   }
-  acc = block_reduce_sum(acc);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  const double s = block_reduce_sum(acc[0] + acc[1]);
+  if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// Sum of the partials over a workgroup of kListThreads, in the same order wherever it is taken; valid in thread 0
-M355_DEV double sum_partials(const double* __restrict__ partials, int count) {
-  double acc = 0.0;
-  for (int i = threadIdx.x; i < count; i += kListThreads) acc += partials[i];
-  return block_reduce_sum(acc);
+// Sum over a workgroup of kFinalThreads; valid in thread 0
+M355_DEV double sum_wide(double v) {
+  __shared__ double red[kFinalThreads / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int w = 1; w < kFinalThreads / 64; ++w) v += red[w];
+  return v;
 }
 
 M355_DEV void store_norm(void* norm, int dtype, double v) {
@@ -112,39 +119,53 @@ M355_DEV void store_norm(void* norm, int dtype, double v) {
   else *static_cast<float*>(norm) = (float)v;
 }
 
-__global__ __launch_bounds__(kListThreads) void k_norm_final(const double* __restrict__ partials, int count,
-                                                             double* __restrict__ sumsq, void* __restrict__ norm,
-                                                             int norm_dtype) {
-  const double s = sum_partials(partials, count);
+// Joins the partial sums: the sum of squares, the norm, and the factor of the clipping (1: nothing is clipped)
+__global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __restrict__ partials, int count,
+                                                              double* __restrict__ sumsq, void* __restrict__ norm,
+                                                              int norm_dtype, double max_norm, double* __restrict__ factor) {
+  double acc = 0.0;
+  for (int base = threadIdx.x; base < count; base += 4 * kFinalThreads) {
+    double v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = base + j * kFinalThreads < count ? partials[base + j * kFinalThreads] : 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc += v[j];
+  }
+  const double s = sum_wide(acc);
   if (threadIdx.x == 0) {
+    const double n = ::sqrt(s);
     if (sumsq) *sumsq = s;
-    store_norm(norm, norm_dtype, ::sqrt(s));
+    store_norm(norm, norm_dtype, n);
+    if (factor) *factor = n > max_norm && n < kInf ? max_norm / n : 1.0;
   }
 }
 
-// Every workgroup adds the partials itself (a few reads from L2), so that norm and scale need no launch in between.
-__global__ __launch_bounds__(kListThreads) void k_norm_scale(const TensorList l, const double* __restrict__ partials,
-                                                             int count, double max_norm, void* __restrict__ norm,
-                                                             int norm_dtype) {
-  __shared__ double shared_sum;
-  const double s = sum_partials(partials, count);
-  if (threadIdx.x == 0) {
-    shared_sum = s;
-    if (blockIdx.x == 0) store_norm(norm, norm_dtype, ::sqrt(s));
-  }
-  __syncthreads();
-  const double n = ::sqrt(shared_sum);
-  const bool clips = n > max_norm && n < kInf;
-  const double f = clips ? max_norm / n : 1.0;
+// One workgroup per chunk.  The list comes with its last tensors first: they are what the Infinity Cache still holds of the
+// pass that formed the norm.
+template <class T> __global__ __launch_bounds__(kListThreads) void k_norm_scale(const TensorList l, const double* __restrict__ factor) {
+  constexpr int N = kPer<T>;
+  typedef typename T::comp comp;
+  const double f = *factor;
   for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
     const int t = tensor_of(l, c);
-    if (!clips && l.in[t] == l.out[t]) continue;
-    const long long i = c - l.first[t];
-    switch (l.dtype[t]) {
-      case M355_F64: scale_chunk<F64>(l.in[t], l.out[t], l.n[t], i * kChunkElems<F64>, f); break;
-      case M355_F32: scale_chunk<F32>(l.in[t], l.out[t], l.n[t], i * kChunkElems<F32>, f); break;
-      case M355_F16: scale_chunk<F16>(l.in[t], l.out[t], l.n[t], i * kChunkElems<F16>, f); break;
-      default: scale_chunk<BF16>(l.in[t], l.out[t], l.n[t], i * kChunkElems<BF16>, f); break;
+    if (f == 1.0 && l.in[t] == l.out[t]) continue;  // in place and not clipped
+    const Chunk<T> k(l, t, c);
+    typename T::store* out = static_cast<typename T::store*>(l.out[t]);
+    raw_t<T> raw[kChunkVecs];
+#pragma unroll
+    for (int j = 0; j < kChunkVecs; ++j)
+      if (k.whole(j)) raw[j] = load_raw_nt<T>(k.p + k.at + (long long)j * kListThreads * N);
+    const long long e = k.tail(l, t, c);
+    if (e >= 0) out[e] = (typename T::store)(comp)((double)k.p[e] * f);
+#pragma unroll
+    for (int j = 0; j < kChunkVecs; ++j) {
+      if (!k.whole(j)) continue;
+      comp v[N];
+      unpack<T>(raw[j], v);
+      // the product in float64, rounded to float32 on the way to a 16-bit type (which is off by at most 2^-24 more)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (comp)((double)v[i] * f);
+      store_raw_nt<T>(out + k.at + (long long)j * kListThreads * N, pack<T>(v));
     }
   }
 }
@@ -163,16 +184,12 @@ int launched() {
 
 size_t item_size(int dtype) { return dtype == M355_F64 ? 8 : dtype == M355_F32 ? 4 : 2; }
 
-long long chunk_elems(int dtype) {
-  return (long long)m355::kListThreads * m355::kChunkVecs * (16 / (long long)item_size(dtype));
-}
-
 int check_list(int64_t count, const m355_tensor* t, bool out) {
   if (count < 0 || (count && !t)) return fail(M355_ERR_INVALID, "bad list of tensors");
   for (int64_t i = 0; i < count; ++i) {
     if (t[i].dtype != M355_F64 && t[i].dtype != M355_F32 && t[i].dtype != M355_F16 && t[i].dtype != M355_BF16)
       return fail(M355_ERR_INVALID, "tensor %lld: float64, float32, float16 or bfloat16", (long long)i);
-    if (t[i].n < 0 || t[i].n > INT64_C(1) << 42) return fail(M355_ERR_INVALID, "tensor %lld: bad size", (long long)i);
+    if (t[i].n < 0 || t[i].n > INT64_C(1) << 40) return fail(M355_ERR_INVALID, "tensor %lld: bad size", (long long)i);
     if (t[i].n && (!t[i].ptr || (out && !t[i].out))) return fail(M355_ERR_INVALID, "NULL pointer argument");
   }
   return 0;
@@ -203,49 +220,62 @@ int check_overlap(int64_t count, const m355_tensor* t) {
   return 0;
 }
 
-// Calls f(list) for launch-sized pieces of the tensors that are not empty.
-template <class F> void each_launch(int64_t count, const m355_tensor* t, F f) {
-  TensorList l;
-  l.count = 0;
-  l.chunks = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    const long long ce = chunk_elems(t[i].dtype);
-    long long at = 0;
-    while (at < t[i].n) {  // a launch counts its chunks in 31 bits: a tensor that would not fit goes on in the next one
-      if (l.count == kListMax || l.chunks >= (1 << 30)) {
-        f(l);
-        l.count = l.chunks = 0;
-      }
-      const long long room = (1ll << 30) - l.chunks;
-      const long long n = std::min((long long)t[i].n - at, room * ce);
-      const size_t off = (size_t)at * item_size(t[i].dtype);
-      l.in[l.count] = static_cast<const char*>(t[i].ptr) + off;
-      l.out[l.count] = t[i].out ? static_cast<char*>(t[i].out) + off : nullptr;
-      l.n[l.count] = n;
-      l.first[l.count] = l.chunks;
-      l.dtype[l.count] = (unsigned char)t[i].dtype;
-      l.chunks += (int)((n + ce - 1) / ce);
-      ++l.count;
-      at += n;
-    }
+template <class F> void by_dtype(int dtype, F f) {
+  switch (dtype) {
+    case M355_F64: return f(m355::F64());
+    case M355_F32: return f(m355::F32());
+    case M355_F16: return f(m355::F16());
+    default: return f(m355::BF16());
   }
-  if (l.count) f(l);
 }
 
-// launches of a list: what the workspace is sized for (each tensor may be continued in one more launch)
-int64_t launches_of(int64_t count) { return (count + kListMax - 1) / kListMax + 1; }
+// Calls f(type, list) for launch-sized pieces of the tensors that are not empty, type by type; backwards: the last first.
+template <class F> void each_launch(int64_t count, const m355_tensor* t, bool backwards, F f) {
+  const int types[4] = {M355_F64, M355_F32, M355_F16, M355_BF16};
+  bool has[5] = {};
+  for (int64_t i = 0; i < count; ++i)
+    if (t[i].n) has[t[i].dtype] = true;
+  for (int step = 0; step < 4; ++step) {
+    const int dtype = types[backwards ? 3 - step : step];
+    if (!has[dtype]) continue;
+    by_dtype(dtype, [&](auto type) {
+      TensorList l;
+      l.count = l.chunks = 0;
+      const long long ce = m355::kChunkElems<decltype(type)>;
+      for (int64_t at = 0; at < count; ++at) {
+        const m355_tensor& x = t[backwards ? count - 1 - at : at];
+        if (x.dtype != dtype || !x.n) continue;
+        const int chunks = (int)((x.n + ce - 1) / ce);  // at most 2^30 (check_list)
+        if (l.count == kListMax || l.chunks > INT32_MAX - chunks) {
+          f(type, l);
+          l.count = l.chunks = 0;
+        }
+        l.in[l.count] = x.ptr;
+        l.out[l.count] = x.out;
+        l.n[l.count] = x.n;
+        l.first[l.count] = l.chunks;
+        l.chunks += chunks;
+        ++l.count;
+      }
+      if (l.count) f(type, l);
+    });
+  }
+}
+
+// launches of a list at most: full ones, one begun per type, and what a launch's chunk count (31 bits) cuts off
+int64_t launches_of(int64_t count) { return count / kListMax + 4; }
 
 int partial_sums(int64_t count, const m355_tensor* t, double* ws, size_t ws_bytes, hipStream_t s, int* nparts) {
-  const size_t room = ws_bytes / sizeof(double);
+  const size_t room = ws_bytes / sizeof(double) - 1;  // one double stays free for the factor
   size_t at = 0;
   bool fits = true;
-  each_launch(count, t, [&](const TensorList& l) {
+  each_launch(count, t, false, [&](auto type, const TensorList& l) {
     const int grid = l.chunks < m355::kNormBlocks ? l.chunks : m355::kNormBlocks;
-    if (!fits || at + grid >= room) {  // one double stays free for the joined sum
+    if (!fits || at + grid > room) {
       fits = false;
       return;
     }
-    hipLaunchKernelGGL(m355::k_norm_partials, dim3(grid), dim3(m355::kListThreads), 0, s, l, ws + at);
+    hipLaunchKernelGGL((m355::k_norm_partials<decltype(type)>), dim3(grid), dim3(m355::kListThreads), 0, s, l, ws + at);
     at += grid;
   });
   *nparts = (int)at;
@@ -254,7 +284,7 @@ int partial_sums(int64_t count, const m355_tensor* t, double* ws, size_t ws_byte
 }  // namespace
 
 extern "C" size_t m355_global_norm_workspace_bytes(int64_t count) {
-  return (size_t)launches_of(count > 0 ? count : 0) * m355::kNormBlocks * sizeof(double);
+  return ((size_t)launches_of(count > 0 ? count : 0) * m355::kNormBlocks + 1) * sizeof(double);
 }
 
 extern "C" int m355_global_norm(int64_t count, const m355_tensor* tensors, double* sumsq, void* norm, int norm_dtype,
@@ -268,7 +298,8 @@ extern "C" int m355_global_norm(int64_t count, const m355_tensor* tensors, doubl
   double* ws = static_cast<double*>(workspace);
   int nparts = 0;
   if ((rc = partial_sums(count, tensors, ws, workspace_bytes, s, &nparts))) return rc;
-  hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kListThreads), 0, s, ws, nparts, sumsq, norm, norm_dtype);
+  hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kFinalThreads), 0, s, ws, nparts, sumsq, norm, norm_dtype,
+                     0.0, static_cast<double*>(nullptr));
   return launched();
 }
 
@@ -278,9 +309,8 @@ extern "C" int m355_clip_global_norm(int64_t count, const m355_tensor* tensors, 
   if (rc) return rc;
   if (!(max_norm >= 0.0)) return fail(M355_ERR_INVALID, "max_norm must be >= 0");
   if (norm_dtype != M355_F64 && norm_dtype != M355_F32) return fail(M355_ERR_INVALID, "the norm is float64 or float32");
-  if (!sumsq && !workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
-  if (!sumsq && workspace_bytes < m355_global_norm_workspace_bytes(count))
-    return fail(M355_ERR_WORKSPACE, "workspace too small");
+  if (!workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (workspace_bytes < m355_global_norm_workspace_bytes(count)) return fail(M355_ERR_WORKSPACE, "workspace too small");
   try {
     if ((rc = check_overlap(count, tensors))) return rc;
   } catch (const std::bad_alloc&) {
@@ -288,26 +318,13 @@ extern "C" int m355_clip_global_norm(int64_t count, const m355_tensor* tensors, 
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   double* ws = static_cast<double*>(workspace);
-  const double* parts = sumsq;
-  int nparts = 1;
-  if (!sumsq) {
-    if ((rc = partial_sums(count, tensors, ws, workspace_bytes, s, &nparts))) return rc;
-    parts = ws;
-    if (nparts > m355::kNormBlocks) {  // several launches: one workgroup adds their partials, not every workgroup of the scale
-      hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kListThreads), 0, s, ws, nparts, ws + nparts, nullptr,
-                         M355_F64);
-      parts = ws + nparts;
-      nparts = 1;
-    }
-  }
-  bool first = true;
-  each_launch(count, tensors, [&](const TensorList& l) {
-    const int grid = l.chunks < 8192 ? l.chunks : 8192;
-    hipLaunchKernelGGL(m355::k_norm_scale, dim3(grid), dim3(m355::kListThreads), 0, s, l, parts, nparts, max_norm,
-                       first ? norm : nullptr, norm_dtype);
-    first = false;
+  int nparts = 0;
+  if (!sumsq && (rc = partial_sums(count, tensors, ws, workspace_bytes, s, &nparts))) return rc;
+  double* factor = ws + nparts;
+  hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kFinalThreads), 0, s, sumsq ? sumsq : ws, sumsq ? 1 : nparts,
+                     static_cast<double*>(nullptr), norm, norm_dtype, max_norm, factor);
+  each_launch(count, tensors, true, [&](auto type, const TensorList& l) {
+    hipLaunchKernelGGL((m355::k_norm_scale<decltype(type)>), dim3(l.chunks), dim3(m355::kListThreads), 0, s, l, factor);
   });
-  if (first)  // nothing to scale: the norm alone
-    hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kListThreads), 0, s, parts, nparts, nullptr, norm, norm_dtype);
   return launched();
 }
