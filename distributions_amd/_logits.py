@@ -4,47 +4,67 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 from math import prod
 
 import numpy as np
 
 from . import _lib
-from ._dispatch import _device_of, _is_torch, _shape_of, _torch
+from ._dispatch import _device_of
+from ._dispatch import _torch as _check_torch
 from ._lib import BF16, F16, F32, F64, I32, I64, LogitAdjust, Operand
 
+_L = _torch_module = None
 _codes = None  # torch dtype -> code of the types logits may have
-_bound = False
+_x_codes = None  # ... observations may have
 _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 MASK_NONE, MASK_BYTES, MASK_BITS = 0, 1, 2
+# Calls of a few microseconds on the GPU come one after the other here, so the C structs are packed in one go: filling them
+# field by field took longer than the kernels.
+_OPERAND = "Qdqqii"
+_pack_operand = struct.Struct("=" + _OPERAND).pack
+_pack_adjust = struct.Struct("=QqqQQQqQqiiii" + 4 * _OPERAND).pack
+assert struct.calcsize("=" + _OPERAND) == ctypes.sizeof(Operand)
+assert struct.calcsize("=QqqQQQqQqiiii" + 4 * _OPERAND) == ctypes.sizeof(LogitAdjust)
 
 
 def _bind():
-    global _bound, _codes
-    L = _lib.lib()
-    if not _bound:
-        import torch
-
-        ap, op = ctypes.POINTER(LogitAdjust), ctypes.POINTER(Operand)
+    """(torch, library), the argument types declared; raises without a GPU or the library."""
+    global _L, _torch_module, _codes, _x_codes
+    if _L is None:
+        torch = _check_torch()
+        L = _lib.lib()
+        bp = ctypes.c_char_p  # a packed struct
         L.m355_logits_adjust.restype = _i32
-        L.m355_logits_adjust.argtypes = [_i64, _i64, _i32, _vp, _i64, ap, _vp, _i64, _vp]
+        L.m355_logits_adjust.argtypes = [_i64, _i64, _i32, _vp, _i64, bp, _vp, _i64, _vp]
         L.m355_logits_adjust_grad_workspace_bytes.restype = _sz
         L.m355_logits_adjust_grad_workspace_bytes.argtypes = [_i64, _i64, _i32]
         L.m355_logits_adjust_grad.restype = _i32
-        L.m355_logits_adjust_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i64, ap, _vp, _vp, _vp, _sz, _vp]
+        L.m355_logits_adjust_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i64, bp, _vp, _vp, _vp, _sz, _vp]
         L.m355_logits_workspace_bytes.restype = _sz
         L.m355_logits_workspace_bytes.argtypes = [_i64, _i64, _i32]
         L.m355_logits_logpdf.restype = _i32
         L.m355_logits_logpdf.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _vp, _sz, _vp]
         L.m355_logits_sum_logpdf_grad.restype = _i32
-        L.m355_logits_sum_logpdf_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, op, _vp, _vp, _i64, _vp, _sz, _vp]
+        L.m355_logits_sum_logpdf_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, bp, _vp, _vp, _i64, _vp, _sz, _vp]
         _codes = {torch.float64: F64, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        _bound = True
-    return L
+        _x_codes = {torch.int64: I64, torch.int32: I32, torch.float64: F64, torch.float32: F32}
+        _torch_module, _L = torch, L
+    return _torch_module, _L
+
+
+def _stream(torch, device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _device(logits, args, torch):
+    """The logits' device if they are on a GPU, else that of the first argument that is."""
+    return logits.device if isinstance(logits, torch.Tensor) and logits.is_cuda else _device_of(args, torch)
 
 
 def _tensor(a, torch, device):
     """A CUDA tensor of `a`'s own dtype (Python numbers and lists: what NumPy makes of them)."""
-    if _is_torch(a):
+    if isinstance(a, torch.Tensor):
         return a if a.device == device else a.to(device)
     return torch.from_numpy(np.array(np.asarray(a), order="C", copy=True)).to(device)
 
@@ -73,20 +93,17 @@ def _rows(t):
 
 
 def _is_number(a):
-    return isinstance(a, (float, int, np.floating, np.integer)) and not isinstance(a, bool)
+    return type(a) is float or type(a) is int or (isinstance(a, (float, int, np.floating, np.integer)) and not isinstance(a, bool))
 
 
-def _row_operand(o, a, batch, torch, device, keep, what, positive=False):
-    """Fill Operand `o` with a per-row argument: a number, or an array that broadcasts to the rows' shape."""
-    o.div = o.mod = 1
-    o.reserved = 0
+def _row_operand(a, batch, torch, device, keep, what, positive=False):
+    """The fields of an Operand from a per-row argument: a number, or an array that broadcasts to the rows' shape."""
     if _is_number(a):
         if positive and not a > 0:
             raise ValueError(f"{what} must be positive, got {a}")
-        o.ptr, o.scalar, o.dtype = None, float(a), F64
-        return
+        return 0, float(a), 1, 1, F64, 0
     t = _tensor(a, torch, device)
-    if t.dtype not in (torch.float64, torch.float32):
+    if t.dtype is not torch.float32 and t.dtype is not torch.float64:
         t = t.to(torch.float64)
     if t.shape != batch:
         try:
@@ -99,17 +116,17 @@ def _row_operand(o, a, batch, torch, device, keep, what, positive=False):
             t = t.expand(batch)
     t = t.contiguous()
     keep.append(t)
-    o.ptr, o.scalar, o.dtype, o.mod = t.data_ptr(), 0.0, F64 if t.dtype == torch.float64 else F32, max(t.numel(), 1)
+    return t.data_ptr(), 0.0, 1, max(t.numel(), 1), F32 if t.dtype is torch.float32 else F64, 0
 
 
 def _row_ints(a, batch, torch, device, keep, what):
-    """Pointer to int64 values, one per row, or None."""
+    """Pointer to int64 values, one per row, or 0."""
     if a is None:
-        return None
+        return 0
     t = _tensor(a, torch, device)
-    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        raise TypeError(f"{what}: integers, got {t.dtype}")
-    if t.dtype != torch.int64:
+    if t.dtype is not torch.int64:
+        if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+            raise TypeError(f"{what}: integers, got {t.dtype}")
         t = t.to(torch.int64)
     if t.shape != batch:
         try:
@@ -126,11 +143,12 @@ def _wide_rows(t, batch, width, keep, what):
     share it."""
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError(f"{what}: the last axis must have {width} entries, got shape {tuple(t.shape)}")
-    if prod(t.shape[:-1]) == 1:
+    lead = t.shape[:-1]
+    if prod(lead) == 1:
         t = t.reshape(width).contiguous()
         keep.append(t)
         return t, 0
-    if t.shape[:-1] != batch:
+    if lead != batch:
         try:
             t = t.expand(tuple(batch) + (width,))
         except RuntimeError:
@@ -142,13 +160,14 @@ def _wide_rows(t, batch, width, keep, what):
 
 def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths, repetition, presence, frequency, bias,
                 temperature, mask):
-    """The C struct of an adjustment, the tensors it points to, and the bias as given (tensor or None)."""
+    """The C struct of an adjustment (packed), the tensors it points to, the bias as given (tensor or None) and whether all
+    rows share it."""
     keep = []
-    d = LogitAdjust()
-    _row_operand(d.repetition, repetition, batch, torch, device, keep, "repetition", positive=True)
-    _row_operand(d.presence, presence, batch, torch, device, keep, "presence")
-    _row_operand(d.frequency, frequency, batch, torch, device, keep, "frequency")
-    _row_operand(d.temperature, temperature, batch, torch, device, keep, "temperature", positive=True)
+    rep = _row_operand(repetition, batch, torch, device, keep, "repetition", positive=True)
+    pres = _row_operand(presence, batch, torch, device, keep, "presence")
+    freq = _row_operand(frequency, batch, torch, device, keep, "frequency")
+    temp = _row_operand(temperature, batch, torch, device, keep, "temperature", positive=True)
+    hist = hist_len = hist_stride = hist_code = lens = prompts = 0
     if history is None:
         if lengths is not None or prompt_lengths is not None:
             raise ValueError("lengths and prompt_lengths belong to a history")
@@ -157,37 +176,41 @@ def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths
                 raise ValueError(f"{what} needs a history")
     else:
         h = _tensor(history, torch, device)
-        if h.dtype not in (torch.int64, torch.int32):
-            if h.is_floating_point() or h.is_complex() or h.dtype == torch.bool:
+        if h.dtype is not torch.int64 and h.dtype is not torch.int32:
+            if h.is_floating_point() or h.is_complex() or h.dtype is torch.bool:
                 raise TypeError(f"history: integer ids, got {h.dtype}")
             h = h.to(torch.int64)
         if h.dim() < 1:
             raise ValueError("history: shape (..., n)")
-        if h.shape[-1] >= 1 << 31:
+        hist_len = h.shape[-1]
+        if hist_len >= 1 << 31:
             raise ValueError("history: fewer than 2**31 ids per row")
-        h, d.history_stride = _wide_rows(h, batch, h.shape[-1], keep, "history")
-        d.history, d.history_len = h.data_ptr(), h.shape[-1]
-        d.history_dtype = I64 if h.dtype == torch.int64 else I32
-        d.lengths = _row_ints(lengths, batch, torch, device, keep, "lengths")
-        d.prompt_lengths = _row_ints(prompt_lengths, batch, torch, device, keep, "prompt_lengths")
+        h, hist_stride = _wide_rows(h, batch, hist_len, keep, "history")
+        hist, hist_code = h.data_ptr(), I64 if h.dtype is torch.int64 else I32
+        lens = _row_ints(lengths, batch, torch, device, keep, "lengths")
+        prompts = _row_ints(prompt_lengths, batch, torch, device, keep, "prompt_lengths")
     given = None
+    bias_ptr = bias_stride = bias_code = 0
     if bias is not None:
         given = b = _tensor(bias, torch, device)
-        if b.dtype != dtype and not (b.dtype == torch.float32 and dtype != torch.float64):
-            given = b = b.to(torch.float64 if dtype == torch.float64 else torch.float32)
-        b, d.bias_stride = _wide_rows(b, batch, k, keep, "bias")
-        d.bias, d.bias_dtype = b.data_ptr(), _codes[b.dtype]
+        if b.dtype is not dtype and not (b.dtype is torch.float32 and dtype is not torch.float64):
+            given = b = b.to(torch.float64 if dtype is torch.float64 else torch.float32)
+        b, bias_stride = _wide_rows(b, batch, k, keep, "bias")
+        bias_ptr, bias_code = b.data_ptr(), _codes[b.dtype]
+    mask_ptr = mask_stride = mask_kind = 0
     if mask is not None:
         m = _tensor(mask, torch, device)
-        if m.dtype == torch.bool:
-            d.mask_kind, width = MASK_BYTES, k
-        elif m.dtype == torch.int32:
-            d.mask_kind, width = MASK_BITS, (k + 31) // 32
+        if m.dtype is torch.bool:
+            mask_kind, width = MASK_BYTES, k
+        elif m.dtype is torch.int32:
+            mask_kind, width = MASK_BITS, (k + 31) // 32
         else:
             raise TypeError(f"mask: bool (one per category) or int32 (32 categories a word), got {m.dtype}")
-        m, d.mask_stride = _wide_rows(m, batch, width, keep, "mask")
-        d.mask = m.data_ptr()
-    return d, keep, given
+        m, mask_stride = _wide_rows(m, batch, width, keep, "mask")
+        mask_ptr = m.data_ptr()
+    packed = _pack_adjust(hist, hist_len, hist_stride, lens, prompts, bias_ptr, bias_stride, mask_ptr, mask_stride, hist_code,
+                          bias_code, mask_kind, 0, *rep, *pres, *freq, *temp)
+    return packed, keep, given, bias_stride == 0
 
 
 def _span(t):
@@ -198,7 +221,7 @@ def _span(t):
 
 def _out_rows(out, z, inputs, torch):
     """Checks a caller's output for logits `z` (2-d rows, their stride): returns its rows and stride."""
-    if not _is_torch(out) or out.dtype != z.dtype or out.device != z.device:
+    if not isinstance(out, torch.Tensor) or out.dtype != z.dtype or out.device != z.device:
         raise ValueError("out: a tensor of the logits' dtype on their device")
     if tuple(out.shape) != tuple(inputs[0].shape):
         raise ValueError(f"out has shape {tuple(out.shape)}, the logits {tuple(inputs[0].shape)}")
@@ -238,66 +261,62 @@ class _on:
 
 
 def adjust(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask, out):
-    torch = _torch()
-    L = _bind()
+    torch, L = _bind()
     args = (logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask)
-    device = _device_of(args, torch)
-    want_torch = out is not None or any(_is_torch(a) for a in args)
+    device = _device(logits, args, torch)
     with _on(torch, device):
         t = _logits(logits, torch, device)
-        batch, k = t.shape[:-1], t.shape[-1]
+        shape = t.shape
+        k = shape[-1]
         z, stride = _rows(t)
-        d, keep, _ = _adjustment(batch, k, z.dtype, torch, device, history, lengths, prompt_lengths, repetition, presence,
-                                 frequency, bias, temperature, mask)
+        d, keep, _, _ = _adjustment(shape[:-1], k, z.dtype, torch, device, history, lengths, prompt_lengths, repetition, presence,
+                                    frequency, bias, temperature, mask)
         if out is None:
-            res = torch.empty(t.shape, dtype=z.dtype, device=device)
+            res = torch.empty(shape, dtype=z.dtype, device=device)
             o, ostride = res, k
         else:
             res = out
             o, ostride = _out_rows(out, z, [t] + keep, torch)
         if z.shape[0]:
-            _lib.check(L.m355_logits_adjust(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, ctypes.byref(d),
-                                            o.data_ptr(), ostride, torch.cuda.current_stream(device).cuda_stream))
+            _lib.check(L.m355_logits_adjust(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, d, o.data_ptr(), ostride,
+                                            _stream(torch, device)))
         del keep
-    return res if want_torch else res.cpu().numpy()
+    return res if out is not None or any(isinstance(a, torch.Tensor) for a in args) else res.cpu().numpy()
 
 
 def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask):
-    torch = _torch()
-    L = _bind()
+    torch, L = _bind()
     args = (g, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask)
-    device = _device_of(args, torch)
-    want_torch = any(_is_torch(a) for a in args)
+    device = _device(logits, args, torch)
     with _on(torch, device):
         t = _logits(logits, torch, device)
-        batch, k = t.shape[:-1], t.shape[-1]
+        shape = t.shape
+        k = shape[-1]
         z, stride = _rows(t)
         gt = _tensor(g, torch, device)
-        if gt.shape != t.shape:
-            raise ValueError(f"g has shape {tuple(gt.shape)}, the logits {tuple(t.shape)}")
+        if gt.shape != shape:
+            raise ValueError(f"g has shape {tuple(gt.shape)}, the logits {tuple(shape)}")
         gz, gstride = _rows(gt.to(z.dtype))
-        d, keep, b = _adjustment(batch, k, z.dtype, torch, device, history, lengths, prompt_lengths, repetition, presence,
-                                 frequency, bias, temperature, mask)
+        d, keep, b, shared = _adjustment(shape[:-1], k, z.dtype, torch, device, history, lengths, prompt_lengths, repetition,
+                                         presence, frequency, bias, temperature, mask)
         rows, code = z.shape[0], _codes[z.dtype]
-        dz = torch.empty(t.shape, dtype=z.dtype, device=device)
+        dz = torch.empty(shape, dtype=z.dtype, device=device)
         db, ws, need = None, None, 0
         if b is not None:
-            shared = d.bias_stride == 0
-            db = torch.empty(k if shared else t.shape, dtype=b.dtype, device=device)
+            db = torch.empty(k if shared else shape, dtype=b.dtype, device=device)
             if shared:
                 need = L.m355_logits_adjust_grad_workspace_bytes(rows, k, code)
                 ws = torch.empty(need, dtype=torch.uint8, device=device)
                 if not rows:
                     db.zero_()
         if rows:
-            _lib.check(L.m355_logits_adjust_grad(rows, k, code, gz.data_ptr(), gstride, z.data_ptr(), stride,
-                                                 ctypes.byref(d), dz.data_ptr(), None if db is None else db.data_ptr(),
-                                                 None if ws is None else ws.data_ptr(), need,
-                                                 torch.cuda.current_stream(device).cuda_stream))
+            _lib.check(L.m355_logits_adjust_grad(rows, k, code, gz.data_ptr(), gstride, z.data_ptr(), stride, d, dz.data_ptr(),
+                                                 None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+                                                 need, _stream(torch, device)))
         if b is not None:
-            db = db.reshape(b.shape) if d.bias_stride == 0 else _sum_to(db, b.shape)
+            db = db.reshape(b.shape) if shared else _sum_to(db, b.shape)
         del keep
-    if want_torch:
+    if any(isinstance(a, torch.Tensor) for a in args):
         return dz, db
     return dz.cpu().numpy(), None if db is None else db.cpu().numpy()
 
@@ -315,7 +334,7 @@ def _sum_to(t, shape):
 
 def _observations(x, batch, torch, device):
     t = _tensor(x, torch, device)
-    if t.dtype not in (torch.int64, torch.int32, torch.float64, torch.float32):
+    if t.dtype not in _x_codes:
         if t.is_complex():
             raise TypeError("observations are integers or floats")
         t = t.to(torch.float32 if t.is_floating_point() else torch.int64)
@@ -324,19 +343,16 @@ def _observations(x, batch, torch, device):
             t = t.expand(batch)
         except RuntimeError:
             raise ValueError(f"x of shape {tuple(t.shape)} does not broadcast to the rows' shape {tuple(batch)}") from None
-    code = {torch.int64: I64, torch.int32: I32, torch.float64: F64, torch.float32: F32}[t.dtype]
-    return t.contiguous(), code
+    return t.contiguous(), _x_codes[t.dtype]
 
 
 def _value_dtype(z, torch):
-    return torch.float64 if z.dtype == torch.float64 else torch.float32
+    return torch.float64 if z.dtype is torch.float64 else torch.float32
 
 
 def logpdf(x, logits):
-    torch = _torch()
-    L = _bind()
-    device = _device_of((x, logits), torch)
-    want_torch = _is_torch(x) or _is_torch(logits)
+    torch, L = _bind()
+    device = _device(logits, (x, logits), torch)
     with _on(torch, device):
         t = _logits(logits, torch, device)
         batch, k = t.shape[:-1], t.shape[-1]
@@ -346,43 +362,40 @@ def logpdf(x, logits):
         rows, code = z.shape[0], _codes[z.dtype]
         if rows:
             need = L.m355_logits_workspace_bytes(rows, k, code)
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             _lib.check(L.m355_logits_logpdf(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode, out.data_ptr(),
-                                            ws.data_ptr(), need, torch.cuda.current_stream(device).cuda_stream))
-    return out if want_torch else out.cpu().numpy()
+                                            ws.data_ptr() if need else None, need, _stream(torch, device)))
+    return out if isinstance(logits, torch.Tensor) or isinstance(x, torch.Tensor) else out.cpu().numpy()
 
 
 def sum_logpdf(x, logits, weights, grad, out=None):
     """(total, gradient or None) of sum(weights * logpdf(x, logits))."""
-    torch = _torch()
-    L = _bind()
+    torch, L = _bind()
     args = (x, logits, weights)
-    device = _device_of(args, torch)
-    want_torch = out is not None or any(_is_torch(a) for a in args)
+    device = _device(logits, args, torch)
     with _on(torch, device):
         t = _logits(logits, torch, device)
-        batch, k = t.shape[:-1], t.shape[-1]
+        shape = t.shape
+        batch, k = shape[:-1], shape[-1]
         z, stride = _rows(t)
         xt, xcode = _observations(x, batch, torch, device)
         keep = []
-        w = Operand()
-        _row_operand(w, 1.0 if weights is None else weights, batch, torch, device, keep, "weights")
+        w = _pack_operand(*_row_operand(1.0 if weights is None else weights, batch, torch, device, keep, "weights"))
         total = torch.empty((), dtype=_value_dtype(z, torch), device=device)
         rows, code = z.shape[0], _codes[z.dtype]
         dz, o, ostride = None, None, 0
         if grad and out is None:
-            dz = torch.empty(t.shape, dtype=z.dtype, device=device)
+            dz = torch.empty(shape, dtype=z.dtype, device=device)
             o, ostride = dz, k
         elif grad:
             dz = out
             o, ostride = _out_rows(out, z, [t, xt] + keep, torch)
-        need = L.m355_logits_workspace_bytes(rows, k, code)
-        ws = torch.empty(max(need, 8), dtype=torch.uint8, device=device)
-        _lib.check(L.m355_logits_sum_logpdf_grad(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode,
-                                                 ctypes.byref(w), total.data_ptr(),
-                                                 o.data_ptr() if grad and rows else None, ostride, ws.data_ptr(),
-                                                 max(need, 8), torch.cuda.current_stream(device).cuda_stream))
+        need = max(8, L.m355_logits_workspace_bytes(rows, k, code))
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        _lib.check(L.m355_logits_sum_logpdf_grad(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode, w, total.data_ptr(),
+                                                 o.data_ptr() if grad and rows else None, ostride, ws.data_ptr(), need,
+                                                 _stream(torch, device)))
         del keep
-    if want_torch:
+    if out is not None or any(isinstance(a, torch.Tensor) for a in args):
         return total, dz
     return float(total.item()), None if dz is None else dz.cpu().numpy()

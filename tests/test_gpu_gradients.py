@@ -163,6 +163,9 @@ def test_refusals(gpu):
     for grads, out in (([g, g], [g, g]), ([g[:60]], [g[1:61]]), ([g[:50], g[50:]], [g[:50], g[:50]])):
         with pytest.raises(M355Error, match="overlaps"):
             G.clip_global_norm(grads, 1.0, out=out)
+    m = torch.randn(10, 10, device=gpu)
+    with pytest.raises(ValueError, match="gaps"):  # column blocks: their spans interleave
+        G.clip_global_norm([m[:, :6], m[:, 5:]], 1.0, out=[m[:, :6], m[:, 5:]])
     n, _ = G.clip_global_norm([g[:50], g[50:]], 1.0, out=[g[:50], g[50:]])  # neighbours are no overlap
     assert abs(plain_norm([g]) - 1.0) < 1e-6
 

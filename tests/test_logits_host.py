@@ -17,8 +17,15 @@ P = 4096  # a pointer that is never read: every call here is refused or empty
 
 @pytest.fixture(scope="module")
 def L():
-    _gradnorm._bind()
-    return _logits._bind()
+    """The library with the argument types the host layer declares; torch stands in for a GPU (nothing is launched here)."""
+    patch = pytest.MonkeyPatch()
+    for m in (_logits, _gradnorm):
+        patch.setattr(m, "_check_torch", lambda: torch)
+        for n in ("_L", "_torch_module", "_codes"):
+            patch.setattr(m, n, None)
+        lib = m._bind()[1]
+    yield lib
+    patch.undo()
 
 
 def adjustment(**kw):
@@ -32,7 +39,7 @@ def adjustment(**kw):
 
 def test_adjust_refusals(L):
     def call(rows=4, k=10, dtype=F32, z=P, zs=10, d=None, o=P, os=10):
-        return L.m355_logits_adjust(rows, k, dtype, z, zs, ctypes.byref(d if d is not None else adjustment()), o, os, None)
+        return L.m355_logits_adjust(rows, k, dtype, z, zs, bytes(d if d is not None else adjustment()), o, os, None)
 
     assert call(rows=0) == 0
     for kw in (dict(rows=-1), dict(k=0), dict(k=1 << 31), dict(dtype=I64), dict(dtype=9), dict(z=None), dict(o=None), dict(zs=-1),
@@ -49,7 +56,7 @@ def test_adjust_refusals(L):
 
 def test_adjust_grad_refusals(L):
     def call(rows=4, k=10, dtype=F32, g=P, z=P, d=None, dz=P, db=None, ws=P, wsb=1 << 20):
-        return L.m355_logits_adjust_grad(rows, k, dtype, g, 10, z, 10, ctypes.byref(d if d is not None else adjustment()), dz, db, ws, wsb, None)
+        return L.m355_logits_adjust_grad(rows, k, dtype, g, 10, z, 10, bytes(d if d is not None else adjustment()), dz, db, ws, wsb, None)
 
     shared = adjustment(bias=P, bias_dtype=F32)
     need = L.m355_logits_adjust_grad_workspace_bytes(4, 10, F32)
@@ -74,7 +81,7 @@ def test_density_refusals(L):
     assert value(wsb=need - 1) == WORKSPACE
 
     def grad(rows=4, w=one, t=P, dz=P, ds=10, ws=P, wsb=1 << 20):
-        return L.m355_logits_sum_logpdf_grad(rows, 10, F32, P, 10, P, I64, None if w is None else ctypes.byref(w), t, dz, ds, ws, wsb, None)
+        return L.m355_logits_sum_logpdf_grad(rows, 10, F32, P, 10, P, I64, None if w is None else bytes(w), t, dz, ds, ws, wsb, None)
 
     for kw in (dict(w=None), dict(t=None), dict(ds=9), dict(ws=None), dict(w=Operand(P, 0.0, 1, 4, I64, 0))):
         assert grad(**kw) == INVALID, kw
