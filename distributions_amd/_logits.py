@@ -315,10 +315,19 @@ def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presenc
                                                  need, _stream(torch, device)))
         if b is not None:
             db = db.reshape(b.shape) if shared else _sum_to(db, b.shape)
+            if b is not bias and getattr(bias, "dtype", None) is not None:  # it was converted: back to its own type
+                db = db.to(_float_type(bias, db.dtype, torch))
         del keep
     if any(isinstance(a, torch.Tensor) for a in args):
         return dz, db
     return dz.cpu().numpy(), None if db is None else db.cpu().numpy()
+
+
+def _float_type(a, otherwise, torch):
+    """The torch dtype of an array that holds floats of a type the kernels know, else `otherwise`."""
+    dt = a.dtype if isinstance(a, torch.Tensor) else {"float64": torch.float64, "float32": torch.float32,
+                                                      "float16": torch.float16}.get(str(a.dtype))
+    return dt if dt in _codes else otherwise
 
 
 def _sum_to(t, shape):
@@ -390,7 +399,7 @@ def sum_logpdf(x, logits, weights, grad, out=None):
         elif grad:
             dz = out
             o, ostride = _out_rows(out, z, [t, xt] + keep, torch)
-        need = max(8, L.m355_logits_workspace_bytes(rows, k, code))
+        need = L.m355_logits_workspace_bytes(rows, k, code)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         _lib.check(L.m355_logits_sum_logpdf_grad(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode, w, total.data_ptr(),
                                                  o.data_ptr() if grad and rows else None, ostride, ws.data_ptr(), need,

@@ -41,7 +41,8 @@ def adjust(logits, history=None, lengths=None, prompt_lengths=None, repetition=1
 
     history: integer ids (..., n), those outside [0, k) are skipped (padding); lengths, prompt_lengths: integers per row
     (default n and 0; clamped to [0, n]).  repetition, presence, frequency, temperature: numbers or arrays per row.  bias:
-    (k,) or (..., k), of the logits' dtype or float32.  mask: truth values (k,) or (..., k), or int32 words
+    (k,) or (..., k), of the logits' dtype or float32 (other
+    types are converted).  mask: truth values (k,) or (..., k), or int32 words
     (..., ceil(k / 32)) in which category v is bit v % 32 of word v // 32; true / 1 = allowed.  A row that allows nothing is
     all -inf.  out: where the result goes; it may be the logits themselves.  Arrays with leading axes broadcast to
     logits.shape[:-1]."""

@@ -324,7 +324,8 @@ extern "C" int m355_clip_global_norm(int64_t count, const m355_tensor* tensors, 
   hipLaunchKernelGGL(m355::k_norm_final, dim3(1), dim3(m355::kFinalThreads), 0, s, sumsq ? sumsq : ws, sumsq ? 1 : nparts,
                      static_cast<double*>(nullptr), norm, norm_dtype, max_norm, factor);
   each_launch(count, tensors, true, [&](auto type, const TensorList& l) {
-    hipLaunchKernelGGL((m355::k_norm_scale<decltype(type)>), dim3(l.chunks), dim3(m355::kListThreads), 0, s, l, factor);
+    hipLaunchKernelGGL((m355::k_norm_scale<decltype(type)>), dim3(l.chunks < (1 << 23) ? l.chunks : 1 << 23),
+                       dim3(m355::kListThreads), 0, s, l, factor);
   });
   return launched();
 }

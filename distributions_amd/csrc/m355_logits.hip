@@ -123,10 +123,10 @@ M355_DEV void count_history(const AdjustArgs& a, long long row, long long base, 
   long long len = a.lengths ? a.lengths[row] : a.history_len;
   len = len < 0 ? 0 : (len > a.history_len ? a.history_len : len);
   const long long prompt = a.prompts ? a.prompts[row] : 0;
-  for (int first = 0;;) {
+  for (long long first = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = first + u * THREADS + (int)threadIdx.x;
+      const long long i = first + u * THREADS + (int)threadIdx.x;
       const unsigned long long at = (unsigned long long)((long long)id[u] - base);
       if (i < len && at < width) count_one<C>(counts, (unsigned)at, i >= prompt);
     }
@@ -134,7 +134,7 @@ M355_DEV void count_history(const AdjustArgs& a, long long row, long long base, 
     first += U * THREADS;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = (long long)first + u * THREADS + (int)threadIdx.x;
+      const long long i = first + u * THREADS + (int)threadIdx.x;
       id[u] = i < len ? h[i] : (ID)-1;
     }
   }
@@ -264,36 +264,94 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
   }
 }
 
-// Gradient of a bias that all rows share.  A workgroup of kSumGroups x kSumThreads threads takes kSumThreads * kPer columns
-// and a block of rows; a thread owns kPer columns and every kSumGroups-th row of the block, so that the column sums stay in
-// its registers (float64) and kSumRows rows are in flight; the groups are joined in LDS, the row blocks by
-// k_logits_cols_final, all in a fixed order.  Without a history the gradient of the logits is written on the way.
-constexpr int kSumThreads = 128, kSumGroups = 4, kSumRows = 4;
-
-template <class T, bool WRITE>
-__global__ __launch_bounds__(kSumThreads * kSumGroups) void k_logits_adjust_cols(const AdjustArgs a, int chunks,
-                                                                                 int row_blocks, double* __restrict__ partials) {
-  constexpr int N = kPer<T>;
+// Short rows without a history: a thread takes a piece, or the k % kPer last categories, of any row.
+template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_logits_adjust_short(const AdjustArgs a, int pieces) {
   typedef typename T::comp comp;
   typedef typename T::store store;
-  __shared__ double joined[kSumGroups - 1][N][kSumThreads];
-  const int col = threadIdx.x % kSumThreads, group = threadIdx.x / kSumThreads;
+  constexpr int N = kPer<T>;
+  const int nv = (int)(a.k / N), k = (int)a.k;
+  const long long all = a.rows * pieces, step = (long long)gridDim.x * 256;
+  for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < all; p += step) {
+    const long long row = all <= 0xffffffffll ? (unsigned)p / (unsigned)pieces : p / pieces;
+    const int i = (int)(p - row * pieces);
+    const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
+    const comp inv_t = inverse_temperature<comp>(a, row);
+    comp s[N], b[N];
+    bool ok[N];
+    if (i < nv) {
+      unpack<T>(load_raw<T>(src + i * N), s);
+      MaskPiece<T> mask;
+      mask.load(a, row, i * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) ok[e] = mask(a, e);
+      BiasPiece<T, typename std::conditional<BWD, void, B>::type> bias;
+      bias.load(a, row, i * N);
+      bias.add_to(s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int v = i * N + e;
+        if (v >= k) continue;
+        s[e] = (comp)src[v];
+        ok[e] = allowed(a, row, v);
+        if constexpr (!BWD && !std::is_void<B>::value)
+          s[e] += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + v];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int v = i * N + e;
+      if (v < k) b[e] = ok[e] ? s[e] * inv_t : BWD ? (comp)0 : (comp)-kInf;
+    }
+    if constexpr (BWD && !std::is_void<B>::value) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i * N + e < k) static_cast<typename B::store*>(a.dbias)[row * a.k + i * N + e] = (typename B::store)b[e];
+    }
+    if (a.dst) {
+      store* dst = static_cast<store*>(a.dst) + row * a.dst_ld + i * N;
+      if (i < nv) {
+        *reinterpret_cast<raw_t<T>*>(dst) = pack<T>(b);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i * N + e < k) dst[e] = (store)b[e];
+      }
+    }
+  }
+}
+
+// Gradient of a bias that all rows share.  A workgroup of G groups of CT threads takes CT * kPer columns and a block of rows;
+// a thread owns kPer columns and every G-th row of the block, so that the column sums stay in its registers (float64) and
+// kSumRows rows are in flight; the groups are joined in LDS, the row blocks by k_logits_cols_final, all in a fixed order.
+// Without a history the gradient of the logits is written on the way.
+constexpr int kSumThreads = 512, kSumRows = 4;
+
+template <class T, int CT, bool WRITE>
+__global__ __launch_bounds__(kSumThreads) void k_logits_adjust_cols(const AdjustArgs a, int chunks,
+                                                                                 int row_blocks, double* __restrict__ partials) {
+  constexpr int N = kPer<T>;
+  constexpr int G = kSumThreads / CT;
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  __shared__ double joined[G - 1][N][CT];
+  const int col = threadIdx.x % CT, group = threadIdx.x / CT;
   const int nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
   const int chunk = blockIdx.x % chunks, rb = blockIdx.x / chunks;
-  const int i = chunk * kSumThreads + col;  // the piece, or (from nv on) a single category of the tail
+  const int i = chunk * CT + col;  // the piece, or (from nv on) a single category of the tail
   const long long lo = a.rows * rb / row_blocks, hi = a.rows * (rb + 1) / row_blocks;
   double acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.0;
   if (i < nv) {
     const long long v = (long long)i * N;
-    for (long long first = lo + group; first < hi; first += kSumGroups * kSumRows) {
+    for (long long first = lo + group; first < hi; first += G * kSumRows) {
       raw_t<T> raw[kSumRows];
       MaskPiece<T> mask[kSumRows];
       comp inv_t[kSumRows];
 #pragma unroll
       for (int r = 0; r < kSumRows; ++r) {
-        const long long row = first + r * kSumGroups;
+        const long long row = first + r * G;
         if (row >= hi) continue;
         raw[r] = __builtin_nontemporal_load(reinterpret_cast<const raw_t<T>*>(static_cast<const store*>(a.src) + row * a.src_ld + v));
         mask[r].load(a, row, v);
@@ -301,7 +359,7 @@ __global__ __launch_bounds__(kSumThreads * kSumGroups) void k_logits_adjust_cols
       }
 #pragma unroll
       for (int r = 0; r < kSumRows; ++r) {
-        const long long row = first + r * kSumGroups;
+        const long long row = first + r * G;
         if (row >= hi) continue;
         comp s[N];
         unpack<T>(raw[r], s);
@@ -315,7 +373,7 @@ __global__ __launch_bounds__(kSumThreads * kSumGroups) void k_logits_adjust_cols
     }
   } else if (i - nv < tail) {
     const long long v = (long long)nv * N + (i - nv);
-    for (long long row = lo + group; row < hi; row += kSumGroups) {
+    for (long long row = lo + group; row < hi; row += G) {
       const comp s = allowed(a, row, v) ? (comp) static_cast<const store*>(a.src)[row * a.src_ld + v] * inverse_temperature<comp>(a, row)
                                         : (comp)0;
       acc[0] += (double)s;
@@ -328,8 +386,8 @@ __global__ __launch_bounds__(kSumThreads * kSumGroups) void k_logits_adjust_cols
   }
   __syncthreads();
   if (group == 0) {
-#pragma unroll
-    for (int g = 0; g < kSumGroups - 1; ++g)
+#pragma unroll 4
+    for (int g = 0; g < G - 1; ++g)
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] += joined[g][e][col];
     double* out = partials + (long long)rb * a.k;
@@ -482,9 +540,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_grad(const DensityArg
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const store* z = static_cast<const store*>(a.z) + row * a.z_ld;
     store* g = static_cast<store*>(a.grad) + row * a.grad_ld;
-    const comp w = (comp)row_operand(a.weight, row);
+    const double wd = row_operand(a.weight, row);
+    const comp w = (comp)wd;
     const long long xi = observed(a, row);
-    if (w == (comp)0 || xi < 0) {  // the gradient is 0 whatever the row holds: it is not read
+    if (wd == 0.0 || xi < 0) {  // the gradient is 0 whatever the row holds: it is not read
       raw_t<T> none;
       none.x = none.y = none.z = none.w = 0;
       for (int i = tid; i < nv; i += THREADS) __builtin_nontemporal_store(none, reinterpret_cast<raw_t<T>*>(g + (long long)i * N));
@@ -616,6 +675,50 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_grad(const DensityArg
   }
 }
 
+// Short rows (k <= kShort * G): G lanes per row, at most kShort elements a lane, all in registers; a wavefront takes 64 / G
+// rows, there is nothing to wait for but the loads.  10^6 rows of 10 float32: 19 us (value), 31 us (with the gradient).  (A
+// workgroup of 256 threads per short row does little but start: 2 * 10^5 rows of 600 bf16 took 660 us that way, and take
+// 117 us with a wavefront per row.)
+constexpr int kShort = 8;
+template <class T, int G, bool GRAD> __global__ __launch_bounds__(256) void k_logits_short(const DensityArgs a) {
+  typedef typename T::comp comp;
+  typedef typename T::store store;
+  constexpr int kRows = 256 / G;
+  const int l = threadIdx.x % G, k = (int)a.k;
+  for (long long row = (long long)blockIdx.x * kRows + threadIdx.x / G; row < a.rows; row += (long long)gridDim.x * kRows) {
+    const store* z = static_cast<const store*>(a.z) + row * a.z_ld;
+    const long long xi = observed(a, row);
+    const double wd = GRAD ? row_operand(a.weight, row) : 1.0;
+    comp v[kShort];
+#pragma unroll
+    for (int j = 0; j < kShort; ++j) v[j] = j * G + l < k ? (comp)z[j * G + l] : (comp)-kInf;
+    const comp zx = xi >= 0 ? (comp)z[xi] : (comp)0;
+    comp m = v[0];
+#pragma unroll
+    for (int j = 1; j < kShort; ++j) m = max_c(m, v[j]);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) m = max_c(m, (comp)__shfl_xor(m, o, 64));
+    const comp b = finite_max(m);
+    comp s = 0;
+#pragma unroll
+    for (int j = 0; j < kShort; ++j) {
+      v[j] = exp_neg(v[j] - b);
+      s += v[j];
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) s += (comp)__shfl_xor(s, o, 64);
+    if (l == 0) static_cast<comp*>(a.lp)[row] = density(zx, m, s, xi >= 0);
+    if constexpr (GRAD) {
+      store* g = static_cast<store*>(a.grad) + row * a.grad_ld;
+      const bool zero = wd == 0.0 || xi < 0 || s == (comp)0;
+      const comp w = (comp)wd, q = zero ? (comp)0 : -w / s;
+#pragma unroll
+      for (int j = 0; j < kShort; ++j)
+        if (j * G + l < k) g[j * G + l] = (store)(zero ? (comp)0 : v[j] * q + (j * G + l == xi ? w : (comp)0));
+    }
+  }
+}
+
 // Value only: one row per workgroup, tiles of NR 16-byte loads per thread with a running maximum and sum.
 template <class T, int THREADS, int NR>
 __global__ __launch_bounds__(THREADS) void k_logits_value(const DensityArgs a) {
@@ -675,19 +778,23 @@ __global__ __launch_bounds__(THREADS) void k_logits_value(const DensityArgs a) {
   }
 }
 
-// total = sum over rows of w * lp in a fixed order; a row of weight 0 is left out whatever its density
+// total = sum over rows of w * lp in a fixed order; a row of weight 0 is left out whatever its density.  Workgroup b of many
+// sums its share of the rows into partials[b] (lp, weight given), a last one the partials (lp NULL).
+constexpr int kTotalRows = 8192;  // rows from which more than one workgroup sums
+constexpr int kTotalBlocks = 512;
 template <class C>
 __global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp, DevOperand weight, long long rows,
-                                                       C* __restrict__ total) {
+                                                       double* __restrict__ partials, C* __restrict__ total) {
   __shared__ double red[16];
+  const long long lo = rows * blockIdx.x / gridDim.x, hi = rows * (blockIdx.x + 1) / gridDim.x;
   double acc = 0.0;
-  for (long long base = threadIdx.x; base < rows; base += 4096) {
+  for (long long base = lo + threadIdx.x; base < hi; base += 4096) {
     double w[4], v[4];  // four rows' loads together: the launch is all latency
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const long long r = base + j * 1024;
-      w[j] = r < rows ? row_operand(weight, r) : 0.0;
-      v[j] = r < rows ? (double)lp[r] : 0.0;
+      w[j] = r >= hi ? 0.0 : lp ? row_operand(weight, r) : 1.0;
+      v[j] = r >= hi ? 0.0 : lp ? (double)lp[r] : partials[r];
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -699,12 +806,13 @@ __global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp,
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) acc += red[i];
-    total[0] = (C)acc;
+    if (total) total[0] = (C)acc;
+    else partials[blockIdx.x] = acc;
   }
 }
 
 // ---------------------------------------------------------------------------------------------- launches
-constexpr long long kMaxGrid = 1ll << 30;
+constexpr long long kMaxGrid = 1ll << 21;  // workgroups (the launch counts threads in 32 bits); kernels walk on from there
 
 template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   const long long nv = a.k / kPer<T>;
@@ -724,6 +832,13 @@ template <class T, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hi
   // CUs, one piece each (1 x 32768 bf16: 4.9 against 7.1 us).  512 threads halve how often a history is scanned, and cost
   // more than they save (512 x 131072 bf16, 500 ids: 71 against 60 us; 256 x 65536, 8000 ids: 36.8 against 37.6 us).
   const bool few = a.rows * (a.k / kPer<T>) < 256ll * 1024;
+  if (!a.history && a.k / kPer<T> < 256) {  // a workgroup per row would be half empty
+    const int pieces = (int)((a.k + kPer<T> - 1) / kPer<T>);
+    const long long want = (a.rows * pieces + 255) / 256;
+    hipLaunchKernelGGL((k_logits_adjust_short<T, B, BWD>), dim3((unsigned)(want < kMaxGrid ? want : kMaxGrid)), dim3(256), 0,
+                       s, a, pieces);
+    return;
+  }
   if (!a.history) few ? launch_adjust<T, 256, 1, 8, void, B, BWD>(a, s) : launch_adjust<T, 256, 4, 4, void, B, BWD>(a, s);
   else if (a.history_len > 32767) launch_adjust<T, 256, 4, 4, unsigned, B, BWD>(a, s);
   else if (few) launch_adjust<T, 256, 1, 8, unsigned short, B, BWD>(a, s);
@@ -737,23 +852,32 @@ template <class T, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t
   else if constexpr (kPer<T> == 8) launch_adjust<T, F32, BWD>(a, s);
 }
 
-// column chunks and row blocks of k_logits_adjust_cols: about two workgroups per CU, at least kSumGroups * kSumRows rows each
-template <class T> int col_chunks_of(long long k) {
-  return (int)((k / kPer<T> + k % kPer<T> + kSumThreads - 1) / kSumThreads);
-}
-template <class T> int row_blocks_of(long long rows, long long k) {
-  long long rb = 1024 / col_chunks_of<T>(k);
-  if (rb > rows / (kSumGroups * kSumRows)) rb = rows / (kSumGroups * kSumRows);
-  return (int)(rb < 1 ? 1 : rb);
+// Shape of k_logits_adjust_cols: threads per group by the row's length, about four workgroups per CU, at least one round of
+// rows in flight each
+struct ColumnGrid {
+  int ct, chunks, row_blocks;
+};
+template <class T> ColumnGrid column_grid(long long rows, long long k) {
+  const long long columns = k / kPer<T> + k % kPer<T>;  // pieces, and categories of the tail
+  ColumnGrid g;
+  g.ct = columns <= 8 ? 8 : columns <= 32 ? 32 : 128;
+  g.chunks = (int)((columns + g.ct - 1) / g.ct);
+  long long rb = 1024 / g.chunks;
+  const long long most = rows / (kSumThreads / g.ct * kSumRows);
+  if (rb > most) rb = most;
+  g.row_blocks = (int)(rb < 1 ? 1 : rb);
+  return g;
 }
 
 template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, double* ws, hipStream_t s) {
-  const int chunks = col_chunks_of<T>(a.k), rb = row_blocks_of<T>(a.rows, a.k);
-  const dim3 grid((unsigned)((long long)chunks * rb)), block(kSumThreads * kSumGroups);
-  if (a.dst) hipLaunchKernelGGL((k_logits_adjust_cols<T, true>), grid, block, 0, s, a, chunks, rb, ws);
-  else hipLaunchKernelGGL((k_logits_adjust_cols<T, false>), grid, block, 0, s, a, chunks, rb, ws);
-  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + 63) / 64)), dim3(256), 0, s, ws, a.k, rb, dbias,
-                     a.bias_dtype);
+  const ColumnGrid g = column_grid<T>(a.rows, a.k);
+  const dim3 grid((unsigned)((long long)g.chunks * g.row_blocks)), block(kSumThreads);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a, g.chunks, g.row_blocks, ws); };
+  if (g.ct == 8) a.dst ? launch(k_logits_adjust_cols<T, 8, true>) : launch(k_logits_adjust_cols<T, 8, false>);
+  else if (g.ct == 32) a.dst ? launch(k_logits_adjust_cols<T, 32, true>) : launch(k_logits_adjust_cols<T, 32, false>);
+  else a.dst ? launch(k_logits_adjust_cols<T, 128, true>) : launch(k_logits_adjust_cols<T, 128, false>);
+  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + 63) / 64)), dim3(256), 0, s, ws, a.k, g.row_blocks,
+                     dbias, a.bias_dtype);
 }
 
 template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launch_grad(const DensityArgs& a, hipStream_t s) {
@@ -761,16 +885,24 @@ template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launc
                      dim3((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid)), dim3(THREADS), 0, s, a);
 }
 
-// Pieces per thread and threads per workgroup by the row's length.  Measured for bf16 (r + w, 5.1-5.7 TB/s; a copy reaches
+// Lanes per short row; pieces per thread and threads per workgroup by the length of longer ones.  Measured for bf16 (r + w, 5.1-5.7 TB/s; a copy reaches
 // 6.4): four pieces per thread beat eight of half the threads while a row fits 1024 threads (8192 x 32768: 194 against
 // 208 us), then two workgroups of 512 threads a CU beat one of 1024 (4096 x 131072: 415 against 437-450 us) although
 // they read half of the row twice, from the Infinity Cache; rows over 256 KiB take one workgroup a CU again (float32,
 // 1500 x 100003: 256 against 277 us), because the rows of 512 workgroups no longer fit that cache.
+template <class T, int G, bool GRAD> void launch_short(const DensityArgs& a, hipStream_t s) {
+  const long long want = (a.rows * G + 255) / 256;
+  hipLaunchKernelGGL((k_logits_short<T, G, GRAD>), dim3((unsigned)(want < kMaxGrid ? want : kMaxGrid)), dim3(256), 0, s, a);
+}
+
 template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStream_t s) {
   const long long nv = a.k / kPer<T>;
+  if (a.k <= kShort * 4) return launch_short<T, 4, GRAD>(a, s);
+  if (a.k <= kShort * 16) return launch_short<T, 16, GRAD>(a, s);
+  if (a.k <= kShort * 64) return launch_short<T, 64, GRAD>(a, s);
   if constexpr (GRAD) {
     constexpr bool wide = sizeof(typename T::store) == 8;
-    if (nv <= 256 * 2) launch_grad<T, 256, 2, 0, 4, false>(a, s);
+    if (nv <= 64 * 4) launch_grad<T, 64, 4, 0, 4, false>(a, s);
     else if (nv <= 256 * 4) launch_grad<T, 256, 4, 0, wide ? 4 : 8, false>(a, s);
     else if (nv <= 512 * 4) launch_grad<T, 512, 4, 0, 4, false>(a, s);
     else if (nv <= 1024 * 4) launch_grad<T, 1024, 4, 0, wide ? 4 : 8, false>(a, s);
@@ -779,7 +911,9 @@ template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStrea
     else launch_grad<T, 1024, wide ? 6 : 8, wide ? 6 : 4, 4, true>(a, s);
   } else {
     const dim3 grid((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid));
-    if (a.rows >= 1024 || nv <= 256 * 4) hipLaunchKernelGGL((k_logits_value<T, 256, 8>), grid, dim3(256), 0, s, a);
+    if (nv <= 64 * 4) hipLaunchKernelGGL((k_logits_value<T, 64, 4>), grid, dim3(64), 0, s, a);
+    else if (nv <= 256 * 4) hipLaunchKernelGGL((k_logits_value<T, 256, 4>), grid, dim3(256), 0, s, a);
+    else if (a.rows >= 1024) hipLaunchKernelGGL((k_logits_value<T, 256, 8>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_logits_value<T, 1024, 8>), grid, dim3(1024), 0, s, a);
   }
 }
@@ -901,7 +1035,7 @@ extern "C" int m355_logits_adjust(int64_t rows, int64_t k, int dtype, const void
 extern "C" size_t m355_logits_adjust_grad_workspace_bytes(int64_t rows, int64_t k, int dtype) {
   if (rows < 1 || k < 1 || k > INT32_MAX) return 0;
   int rb = 0;
-  m355::by_dtype(dtype, [&](auto t) { return (rb = m355::row_blocks_of<decltype(t)>(rows, k)), 0; });
+  m355::by_dtype(dtype, [&](auto t) { return (rb = m355::column_grid<decltype(t)>(rows, k).row_blocks), 0; });
   return (size_t)rb * (size_t)k * sizeof(double);
 }
 
@@ -917,6 +1051,7 @@ extern "C" int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const
   if (g_stride < 0 || logits_stride < 0) return fail(M355_ERR_INVALID, "bad row stride");
   if (dbias && !a.bias) return fail(M355_ERR_INVALID, "dbias without a bias");
   const bool shared = dbias && a.bias_ld == 0;
+  if (shared && k > (INT64_C(1) << 28)) return fail(M355_ERR_INVALID, "gradient of a shared bias: at most 2^28 categories");
   if (rows == 0 && !shared) return M355_OK;
   if ((rows && (!g || (dlogits && a.history && !logits)))) return fail(M355_ERR_INVALID, "NULL pointer argument");
   if (shared && rows && (!workspace || workspace_bytes < m355_logits_adjust_grad_workspace_bytes(rows, k, dtype)))
@@ -945,7 +1080,7 @@ extern "C" int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const
 extern "C" size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype) {
   (void)k;
   (void)dtype;
-  return (size_t)(rows > 0 ? rows : 0) * sizeof(double);
+  return ((size_t)(rows > 0 ? rows : 0) + m355::kTotalBlocks) * sizeof(double);
 }
 
 extern "C" int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
@@ -974,7 +1109,7 @@ extern "C" int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, c
   if (!weights || !total) return fail(M355_ERR_INVALID, "NULL pointer argument");
   if ((rc = row_arg(*weights, rows, a.weight, "weights"))) return rc;
   if (dlogits && rows > 1 && dlogits_stride < k) return fail(M355_ERR_INVALID, "bad row stride");
-  if (rows && !workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (!workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
   if (workspace_bytes < m355_logits_workspace_bytes(rows, k, dtype)) return fail(M355_ERR_WORKSPACE, "workspace too small");
   a.lp = workspace;
   a.grad = dlogits;
@@ -985,8 +1120,19 @@ extern "C" int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, c
     typedef typename T::comp comp;
     if (rows && dlogits) launch_density<T, true>(a, s);
     else if (rows) launch_density<T, false>(a, s);
-    hipLaunchKernelGGL((k_logits_total<comp>), dim3(1), dim3(1024), 0, s, static_cast<const comp*>(a.lp), a.weight,
-                       (long long)rows, static_cast<comp*>(total));
+    const comp* lp = static_cast<const comp*>(a.lp);
+    comp* out = static_cast<comp*>(total);
+    double* partials = static_cast<double*>(workspace) + rows;  // behind the densities
+    if (rows <= kTotalRows) {
+      hipLaunchKernelGGL((k_logits_total<comp>), dim3(1), dim3(1024), 0, s, lp, a.weight, (long long)rows, partials, out);
+    } else {
+      const long long want = (rows + 4095) / 4096;
+      const int blocks = (int)(want < kTotalBlocks ? want : kTotalBlocks);
+      hipLaunchKernelGGL((k_logits_total<comp>), dim3(blocks), dim3(1024), 0, s, lp, a.weight, (long long)rows, partials,
+                         static_cast<comp*>(nullptr));
+      hipLaunchKernelGGL((k_logits_total<comp>), dim3(1), dim3(1024), 0, s, static_cast<const comp*>(nullptr), a.weight,
+                         (long long)blocks, partials, out);
+    }
     return 0;
   });
   return launched();

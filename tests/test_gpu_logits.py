@@ -327,7 +327,7 @@ def test_out_in_place(gpu):
 
 
 # ------------------------------------------------------------------------------------------------- log-density
-@pytest.mark.parametrize("rows, k", SIZES + [(2, 50021), (1, 131072), (1, 262147), (300, 515), (700, 64)])
+@pytest.mark.parametrize("rows, k", SIZES + [(2, 50021), (1, 131072), (1, 262147), (300, 515), (700, 64), (5, 32), (9, 129), (4, 512), (3, 513)])
 @pytest.mark.parametrize("dt", DT)
 def test_logpdf_total_and_gradient(gpu, dt, rows, k):
     from distributions_amd import categorical_logits as cl
@@ -439,6 +439,56 @@ def test_offsets_past_32_bits(gpu):
     total, (_, g) = cl.sum_logpdf_grad(x, small)
     t2, _ = cl.sum_logpdf_grad(x, z, out=z)
     assert torch.equal(total, t2) and torch.equal(z, g)
+
+
+def test_many_short_rows(gpu):
+    """More rows than the launch has workgroups for one each, k from 1 to the borders of the short kernels."""
+    from distributions_amd import categorical_logits as cl
+
+    for k, dtype in ((1, torch.float32), (10, torch.bfloat16), (32, torch.float64), (33, torch.float32), (300, torch.float16)):
+        rows = 5000
+        z = make((rows, k), dtype, k, gpu)
+        x = torch.arange(rows, device=gpu) % (k + 1) - 1  # one in k + 1 is no category
+        lp, b_lp, _, _, grad, b_g = plain_logpdf(x, z)
+        within(cl.logpdf(x, z), lp, b_lp)
+        _, (_, g) = cl.sum_logpdf_grad(x, z)
+        within(g, grad, b_g)
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        a = adjust_args(rows, k, 3, gpu, 0, "bits", "rows", wide)
+        ref, bound = plain_adjust(z, **a)
+        within(cl.adjust(z, **a), ref, bound)
+        dz, db = cl.adjust_grad(z, z, **a)
+        rz, rb = plain_adjust_grad(z, z, **a)
+        u, ut, tiny = steps(dtype)
+        within(dz, rz, ut * rz.abs() + 6 * u * rz.abs() + tiny)
+        within(db, rb, 3 * u * rb.abs() + 2.0**-149)
+
+
+@pytest.mark.parametrize("k", [20, 3000])
+def test_weights_below_the_arithmetic(gpu, k):
+    """A float64 weight that float32 rounds to 0 is no padding: its row counts in the total."""
+    from distributions_amd import categorical_logits as cl
+
+    z = make((4, k), torch.float32, 2, gpu)
+    x = torch.tensor([0, 1, 2, 3], device=gpu)
+    w = torch.tensor([1.0, 1e-60, 0.0, 2.0], dtype=torch.float64, device=gpu)
+    total, (_, g) = cl.sum_logpdf_grad(x, z, w)
+    lp, b_lp, ref, b_total, grad, b_g = plain_logpdf(x, z, w)
+    within(total, ref, b_total)
+    within(g, grad, b_g)
+
+
+def test_bias_of_another_type(gpu):
+    from distributions_amd import categorical_logits as cl
+
+    z = make((5, 700), torch.float32, 2, gpu)
+    for dtype in (torch.float64, torch.bfloat16, torch.float16):
+        b = make((700,), dtype, 3, gpu)
+        assert torch.equal(cl.adjust(z, bias=b), cl.adjust(z, bias=b.float()))
+        dz, db = cl.adjust_grad(z, z, bias=b)
+        assert db.dtype == dtype and torch.equal(db, cl.adjust_grad(z, z, bias=b.float())[1].to(dtype))
+    dz, db = cl.adjust_grad(z.cpu().numpy(), z.cpu().numpy(), bias=np.zeros(700))
+    assert db.dtype == np.float64
 
 
 def test_numpy_and_types(gpu):
