@@ -109,19 +109,18 @@ def _outputs(ls, out, torch):
     if len(out) != len(ls.grads):
         raise ValueError(f"out has {len(out)} entries, the list of gradients {len(ls.grads)}")
     given = [out[i] for i in ls.places]
+    if not all(isinstance(o, torch.Tensor) for o in given) or {o.device for o in given} - {ls.device}:
+        raise ValueError("out: tensors on the gradients' device")
     outs = []
-    for t, r, o in zip(ls.tensors, ls.runs, given):
-        if o is r:
-            outs.append(o)
-            continue
-        if not isinstance(o, torch.Tensor) or o.dtype is not t.dtype or o.device != t.device or o.shape != t.shape:
-            raise ValueError("out: tensors of the gradients' shapes and dtypes on their device")
-        if (o.is_contiguous() and r.is_contiguous()) or (o.stride() == r.stride() and dense(o)):
-            outs.append(o)
-        else:
-            if any(s == 0 and m > 1 for s, m in zip(o.stride(), o.shape)):
-                raise ValueError("out: elements that share memory")
-            outs.append(torch.empty_like(r))
+    for t, r, o, dt in zip(ls.tensors, ls.runs, given, ls.dtypes):
+        if o is not r:
+            if o.dtype is not dt or o.shape != t.shape:
+                raise ValueError("out: tensors of the gradients' shapes and dtypes")
+            if not (o.is_contiguous() and r.is_contiguous()) and not (o.stride() == r.stride() and dense(o)):
+                if any(s == 0 and m > 1 for s, m in zip(o.stride(), o.shape)):
+                    raise ValueError("out: elements that share memory")
+                o = torch.empty_like(r)
+        outs.append(o)
     for i, (o, r) in enumerate(zip(given, outs)):
         if o is not r and o.numel():  # what the library does not see: it checks the runs it is given
             lo, hi = _span(o)

@@ -122,9 +122,9 @@ def plain_logpdf(x, z, weights=None):
     zx = zz.gather(1, xi)
     empty = (s == 0)[:, 0]
     lp = torch.where(inside & ~empty, (zx - mm - s.log())[:, 0], -INF)
-    # sum of k terms, one after the other at worst over a 64th of the row, then joined: k / 64 + 24 roundings; exp 2^-22
-    # (float64: 2^-50) and the rounding of z - m, which moves the exponent by u |z - m|: weighted by p, at most
-    # u * sum(p |z - m|); log: 2 u |log s|; the two differences: u each
+    # sum of k terms, one after the other at worst over a 64th of the row, then joined: k / 64 + 24 roundings; 2^t itself off
+    # by 2 u (float64 exp: less), and the roundings of z - m, of log2 e and of their product, which move the exponent by less
+    # than 3 u |z - m|: weighted by p, 3 u sum(p |z - m|); log: 2 u |log s|; the two differences: u each
     p = torch.where(s > 0, e / s, 0.0)
     spread = torch.nan_to_num((p * (zz - mm).abs()).sum(1), nan=0.0, posinf=0.0)
     off_s = (k / 64 + 24) * u + 4 * u + 4 * u * spread
