@@ -29,7 +29,7 @@ except ImportError as e:  # pragma: no cover - PyTensor absent here
     raise ImportError("distributions_amd.pytensor_ops needs PyTensor (pip install pytensor); the eager "
                       "functions in distributions_amd.<dist> do not") from e
 
-from . import _catmult, _dispatch, _mv
+from . import _catmult, _dispatch, _logits, _mv
 from ._lib import DISCRETE, FN, GRAD, NPARAMS
 
 
@@ -232,6 +232,49 @@ class M355Categorical(Op):
         return [shapes[0]]
 
 
+class M355LogitsLogpdf(Op):
+    """categorical_logits.logpdf(x, logits): logits (..., k), x broadcasts to their rows, one value per row; float32 for
+    float32 logits, else float64."""
+
+    __props__ = ()
+
+    def make_node(self, x, logits):
+        x, logits = pt.as_tensor_variable(x), pt.as_tensor_variable(logits)
+        if logits.type.ndim < 1 or x.type.ndim > logits.type.ndim - 1:
+            raise ValueError("categorical_logits: logits (..., k), x broadcast to their leading axes")
+        return Apply(self, [x, logits], [pt.tensor(dtype=_out_dtype([logits]), shape=logits.type.shape[:-1])])
+
+    def perform(self, node, inputs, output_storage):
+        output_storage[0][0] = np.asarray(_logits.logpdf(*inputs), dtype=node.outputs[0].dtype)
+
+    def infer_shape(self, fgraph, node, shapes):
+        return [tuple(shapes[1])[:-1]]
+
+    def L_op(self, inputs, outputs, output_grads):
+        return M355LogitsGrad()(*inputs, output_grads[0])
+
+
+class M355LogitsGrad(Op):
+    """(0, g * ([v == x] - softmax(logits)[v])): the gradients of sum(g * logpdf(x, logits)) with respect to x, which is
+    discrete, and the logits, each in the shape of its argument (m355_logits_sum_logpdf_grad)."""
+
+    __props__ = ()
+
+    def make_node(self, x, logits, g):
+        ins = [pt.as_tensor_variable(v) for v in (x, logits, g)]
+        return Apply(self, ins, [pt.tensor(dtype="float64", shape=ins[0].type.shape),
+                                 pt.tensor(dtype=_out_dtype([ins[1]]), shape=ins[1].type.shape)])
+
+    def perform(self, node, inputs, output_storage):
+        x, logits, g = inputs
+        _total, d = _logits.sum_logpdf(x, logits, np.asarray(g), True)
+        output_storage[0][0] = np.zeros(np.shape(x))
+        output_storage[1][0] = np.asarray(d, dtype=node.outputs[1].dtype)
+
+    def infer_shape(self, fgraph, node, shapes):
+        return list(shapes[:2])
+
+
 class M355MultinomialLogpdf(Op):
     """multinomial.logpdf(x, n, p) (multinomial.py:39-54): x (..., k), p (..., k), one value per count vector."""
 
@@ -322,6 +365,9 @@ def symbolic(dist: str) -> types.SimpleNamespace:
         for fn in FN:
             setattr(ns, fn, (lambda f: lambda x, p: M355Categorical(f)(x, p))(fn))
         ns.rvs = _rvs(dist)
+        return ns
+    if dist == "categorical_logits":
+        ns.logpdf = lambda x, logits: M355LogitsLogpdf()(x, logits)
         return ns
     if dist == "multinomial":
         ns.logpdf = lambda x, n, p: M355MultinomialLogpdf()(x, n, p)
