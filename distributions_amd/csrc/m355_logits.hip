@@ -38,13 +38,19 @@ M355_DEV bool allowed(const AdjustArgs& a, long long row, long long v) {
 }
 // The mask of a whole piece (v is a multiple of kPer, v + kPer <= k): the raw bytes resp. the word, then its kPer flags
 template <class T> struct MaskPiece {
-  unsigned long long bytes;
-  M355_DEV void load(const AdjustArgs& a, long long row, long long v) {
-    bytes = ~0ull;
-    if (a.mask_kind == M355_MASK_BYTES)
-      __builtin_memcpy(&bytes, static_cast<const unsigned char*>(a.mask) + row * a.mask_ld + v, kPer<T>);
-    else if (a.mask_kind == M355_MASK_BITS)
-      bytes = static_cast<const unsigned*>(a.mask)[row * a.mask_ld + (v >> 5)] >> (v & 31);
+  typename std::conditional<kPer<T> == 8, unsigned long long, unsigned>::type bytes;
+  // `rel` categories behind category `base` of the row; row and base are the same for the whole workgroup, so that the
+  // address is a scalar plus a 32-bit offset
+  M355_DEV void load(const AdjustArgs& a, long long row, long long base, unsigned rel) {
+    bytes = ~(decltype(bytes))0;
+    if (a.mask_kind == M355_MASK_BYTES) {
+      const unsigned char* m = static_cast<const unsigned char*>(a.mask) + row * a.mask_ld + base;
+      __builtin_memcpy(&bytes, m + rel, kPer<T>);
+    } else if (a.mask_kind == M355_MASK_BITS) {
+      const unsigned* m = static_cast<const unsigned*>(a.mask) + row * a.mask_ld + (base >> 5);
+      const unsigned at = (unsigned)(base & 31) + rel;
+      bytes = m[at >> 5] >> (at & 31);
+    }
   }
   M355_DEV bool operator()(const AdjustArgs& a, int e) const {
     return a.mask_kind == M355_MASK_BYTES ? ((bytes >> (8 * e)) & 0xff) != 0 : ((bytes >> e) & 1) != 0;
@@ -55,10 +61,10 @@ template <class T> struct MaskPiece {
 template <class T, class B> struct BiasPiece {
   static constexpr int kLoads = kPer<T> / kPer<B>;
   raw_t<B> raw[kLoads];
-  M355_DEV void load(const AdjustArgs& a, long long row, long long v) {
+  M355_DEV void load(const AdjustArgs& a, long long row, long long base, unsigned rel) {
+    const typename B::store* b = static_cast<const typename B::store*>(a.bias) + row * a.bias_ld + base;
 #pragma unroll
-    for (int h = 0; h < kLoads; ++h)
-      raw[h] = load_raw<B>(static_cast<const typename B::store*>(a.bias) + row * a.bias_ld + v + h * kPer<B>);
+    for (int h = 0; h < kLoads; ++h) raw[h] = load_raw<B>(b + (rel + h * kPer<B>));
   }
   M355_DEV void add_to(typename T::comp (&s)[kPer<T>]) const {
 #pragma unroll
@@ -71,7 +77,7 @@ template <class T, class B> struct BiasPiece {
   }
 };
 template <class T> struct BiasPiece<T, void> {
-  M355_DEV void load(const AdjustArgs&, long long, long long) {}
+  M355_DEV void load(const AdjustArgs&, long long, long long, unsigned) {}
   M355_DEV void add_to(typename T::comp (&)[kPer<T>]) const {}
 };
 
@@ -110,41 +116,48 @@ template <class C> M355_DEV void count_one(unsigned* counts, unsigned at, bool g
   }
 }
 template <class C, class ID, int THREADS>
-M355_DEV void count_history(const AdjustArgs& a, long long row, long long base, unsigned width, unsigned* counts) {
-  constexpr int U = 8;  // ids in flight per thread: the loop is all latency
+M355_DEV void count_history(const AdjustArgs& a, long long row, unsigned base, unsigned width, unsigned* counts) {
+  constexpr int U = 4;  // ids in flight per thread: the loop is all latency
   const ID* h = static_cast<const ID*>(a.history) + row * a.history_ld;
+  const unsigned most = (unsigned)a.history_len, tid = threadIdx.x;  // positions and ids in 32 bits: both are below 2^31
   // the first ids are fetched before the row's length is known; those behind it are dropped
   ID id[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * THREADS + (int)threadIdx.x;
-    id[u] = i < a.history_len ? h[i] : (ID)-1;
-  }
-  long long len = a.lengths ? a.lengths[row] : a.history_len;
-  len = len < 0 ? 0 : (len > a.history_len ? a.history_len : len);
-  const long long prompt = a.prompts ? a.prompts[row] : 0;
-  for (long long first = 0;;) {
+  for (int u = 0; u < U; ++u) id[u] = u * THREADS + tid < most ? h[u * THREADS + tid] : (ID)-1;
+  const long long given = a.lengths ? a.lengths[row] : a.history_len, start = a.prompts ? a.prompts[row] : 0;
+  const unsigned len = given < 0 ? 0u : given > a.history_len ? most : (unsigned)given;
+  const unsigned prompt = start < 0 ? 0u : start > a.history_len ? most : (unsigned)start;
+  for (unsigned first = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = first + u * THREADS + (int)threadIdx.x;
-      const unsigned long long at = (unsigned long long)((long long)id[u] - base);
-      if (i < len && at < width) count_one<C>(counts, (unsigned)at, i >= prompt);
+      const unsigned i = first + u * THREADS + tid;
+      // an id outside [0, k) lies behind the chunk: base + width is at most 2^31, and a negative one wraps past it
+      const bool small = sizeof(ID) == 4 || (unsigned)((unsigned long long)(long long)id[u] >> 32) == 0;
+      const unsigned at = (unsigned)id[u] - base;
+      if (small && i < len && at < width) count_one<C>(counts, at, i >= prompt);
     }
-    if (first >= len - U * THREADS) break;
     first += U * THREADS;
+    if (first >= len) break;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = first + u * THREADS + (int)threadIdx.x;
+      const unsigned i = first + u * THREADS + tid;
       id[u] = i < len ? h[i] : (ID)-1;
     }
   }
 }
 
-template <class C> M355_DEV C penalised(C s, unsigned count, C rep, C pres, C freq) {
-  if (count) s = s > 0 ? s / rep : s * rep;
-  if (count >> 1) s -= freq * (C)(count >> 1) + pres;
-  return s;
-}
+// The penalties of a row; inv = 1 / rep (one rounding more): a division would be paid for by nearly every wavefront, because
+// nearly every one has some id of the history among its elements (64 x 131072 bf16, 2048 ids: 16.0 us with it, 13.7 without)
+template <class C> struct Penalties {
+  C rep, inv, pres, freq;
+  M355_DEV C factor(C x) const { return x > 0 ? inv : rep; }
+  M355_DEV C operator()(C s, unsigned count) const {
+    const C p = s * factor(s);
+    s = count ? p : s;
+    const C q = s - (freq * (C)(count >> 1) + pres);
+    return count >> 1 ? q : s;
+  }
+};
 
 // One workgroup per (row, chunk): everything the chunk needs from memory is fetched first, then, with a history (CNT: the
 // type of its counters, or void), the ids that fall into the chunk are counted in LDS, then the pieces are worked off.  The
@@ -166,6 +179,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
     if (!item_of(a, grid, item, row, chunk)) continue;
     const int c0 = chunk * grid.per, c1 = c0 + grid.per < nv ? c0 + grid.per : nv;  // pieces of the chunk
     const long long base = (long long)c0 * N;
+    const unsigned count_here = (unsigned)(c1 - c0);
     const bool has_tail = chunk == grid.chunks - 1 && tid < tail;
     const long long vt = (long long)nv * N + tid;
     const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
@@ -174,52 +188,56 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
     BiasPiece<T, typename std::conditional<BWD, void, B>::type> bias[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = c0 + j * THREADS + tid;
-      if (i >= c1) continue;
-      const long long v = (long long)i * N;
-      raw[j] = load_raw<T>(src + v);
-      mask[j].load(a, row, v);
-      bias[j].load(a, row, v);
+      const unsigned i = j * THREADS + tid;
+      if (i >= count_here) continue;
+      raw[j] = load_raw<T>(src + base + i * N);
+      mask[j].load(a, row, base, i * N);
+      bias[j].load(a, row, base, i * N);
     }
-    comp rep = 1, pres = 0, freq = 0;
+    // the row's arguments before the barriers: behind them their latency would stand alone
+    const comp inv_t = inverse_temperature<comp>(a, row);
+    Penalties<comp> penalty = {1, 1, 0, 0};
     if constexpr (HIST) {
+      penalty.rep = (comp)row_operand(a.rep, row);
+      penalty.inv = (comp)1 / penalty.rep;
+      penalty.pres = (comp)row_operand(a.pres, row);
+      penalty.freq = (comp)row_operand(a.freq, row);
       for (int i = tid; i < (int)(sizeof(count_store) / 16); i += THREADS) count_store[i] = uint4{0, 0, 0, 0};
       __syncthreads();
       const long long left = a.k - base;
       const unsigned width = chunk == grid.chunks - 1 ? (unsigned)left : (unsigned)((c1 - c0) * N);
-      if (a.history_dtype == M355_I64) count_history<cnt, long long, THREADS>(a, row, base, width, reinterpret_cast<unsigned*>(counts));
-      else count_history<cnt, int, THREADS>(a, row, base, width, reinterpret_cast<unsigned*>(counts));
+      if (a.history_dtype == M355_I64) count_history<cnt, long long, THREADS>(a, row, (unsigned)base, width, reinterpret_cast<unsigned*>(counts));
+      else count_history<cnt, int, THREADS>(a, row, (unsigned)base, width, reinterpret_cast<unsigned*>(counts));
       __syncthreads();
-      rep = (comp)row_operand(a.rep, row);
-      pres = (comp)row_operand(a.pres, row);
-      freq = (comp)row_operand(a.freq, row);
     }
-    const comp inv_t = inverse_temperature<comp>(a, row);
     store* dst = static_cast<store*>(a.dst) + row * a.dst_ld;
     const store* x = static_cast<const store*>(a.x) + row * a.x_ld;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = c0 + j * THREADS + tid;
-      if (i >= c1) continue;
-      const long long v = (long long)i * N;
+      const unsigned i = j * THREADS + tid, rel = i * N;
+      if (i >= count_here) continue;
       comp s[N];
       unpack<T>(raw[j], s);
       cnt count[N];
       bool any = false;  // most pieces have no id of the history
       if constexpr (HIST) {
-        __builtin_memcpy(count, counts + (i - c0) * N, sizeof(count));
+        __builtin_memcpy(count, counts + rel, sizeof(count));
 #pragma unroll
         for (int e = 0; e < N; ++e) any |= count[e] != 0;
       }
       if constexpr (!BWD) {
         if (any) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) s[e] = penalised<comp>(s[e], count[e], rep, pres, freq);
+          for (int e = 0; e < N; ++e) s[e] = penalty(s[e], count[e]);
         }
         bias[j].add_to(s);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e] = mask[j](a, e) ? s[e] * inv_t : (comp)-kInf;
-        __builtin_nontemporal_store(pack<T>(s), reinterpret_cast<raw_t<T>*>(dst + v));
+        for (int e = 0; e < N; ++e) s[e] *= inv_t;
+        if (a.mask_kind != M355_MASK_NONE) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) s[e] = mask[j](a, e) ? s[e] : (comp)-kInf;
+        }
+        store_raw_nt<T>(dst + base + rel, pack<T>(s));
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) s[e] = mask[j](a, e) ? s[e] * inv_t : (comp)0;
@@ -229,16 +247,16 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
             typename B::comp t[kPer<B>];
 #pragma unroll
             for (int e = 0; e < kPer<B>; ++e) t[e] = (typename B::comp)s[h + e];
-            store_raw_nt<B>(static_cast<typename B::store*>(a.dbias) + row * a.k + v + h, pack<B>(t));
+            store_raw_nt<B>(static_cast<typename B::store*>(a.dbias) + row * a.k + base + (rel + h), pack<B>(t));
           }
         }
         if (a.dst) {
           if (any) {
 #pragma unroll
             for (int e = 0; e < N; ++e)
-              if (count[e]) s[e] = (comp)x[v + e] > 0 ? s[e] / rep : s[e] * rep;
+              if (count[e]) s[e] *= penalty.factor((comp)x[base + (rel + e)]);
           }
-          store_raw_nt<T>(dst + v, pack<T>(s));
+          store_raw_nt<T>(dst + base + rel, pack<T>(s));
         }
       }
     }
@@ -247,7 +265,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
       comp s = (comp)src[vt];
       const bool ok = allowed(a, row, vt);
       if constexpr (!BWD) {
-        s = penalised<comp>(s, count, rep, pres, freq);
+        s = penalty(s, count);
         if constexpr (!std::is_void<B>::value) s += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + vt];
         dst[vt] = (store)(ok ? s * inv_t : (comp)-kInf);
       } else {
@@ -255,7 +273,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustAr
         if constexpr (!std::is_void<B>::value)
           static_cast<typename B::store*>(a.dbias)[row * a.k + vt] = (typename B::store)s;
         if (a.dst) {
-          if (count) s = (comp)x[vt] > 0 ? s / rep : s * rep;
+          if (count) s *= penalty.factor((comp)x[vt]);
           dst[vt] = (store)s;
         }
       }
@@ -281,11 +299,11 @@ template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_l
     if (i < nv) {
       unpack<T>(load_raw<T>(src + i * N), s);
       MaskPiece<T> mask;
-      mask.load(a, row, i * N);
+      mask.load(a, row, 0, i * N);
 #pragma unroll
       for (int e = 0; e < N; ++e) ok[e] = mask(a, e);
       BiasPiece<T, typename std::conditional<BWD, void, B>::type> bias;
-      bias.load(a, row, i * N);
+      bias.load(a, row, 0, i * N);
       bias.add_to(s);
     } else {
 #pragma unroll
@@ -354,7 +372,7 @@ __global__ __launch_bounds__(kSumThreads) void k_logits_adjust_cols(const Adjust
         const long long row = first + r * G;
         if (row >= hi) continue;
         raw[r] = __builtin_nontemporal_load(reinterpret_cast<const raw_t<T>*>(static_cast<const store*>(a.src) + row * a.src_ld + v));
-        mask[r].load(a, row, v);
+        mask[r].load(a, row, 0, (unsigned)v);
         inv_t[r] = inverse_temperature<comp>(a, row);
       }
 #pragma unroll

@@ -58,11 +58,10 @@ def counts_of(history, lengths, prompts, rows, k):
     for r in range(rows):
         last = n if lengths is None else max(0, min(n, int(lengths.reshape(-1)[r])))
         first = 0 if prompts is None else int(prompts.reshape(-1)[r])
-        for i in range(last):
-            v = int(h[r, i])
-            if 0 <= v < k:
-                call[r, v] += 1
-                cgen[r, v] += i >= first
+        for to, ids in ((call, h[r, :last]), (cgen, h[r, max(first, 0) : last])):
+            for v in ids.tolist():
+                if 0 <= v < k:
+                    to[r, v] += 1
     return call, cgen
 
 
@@ -85,8 +84,8 @@ def plain_adjust(z, history=None, lengths=None, prompt_lengths=None, repetition=
         size = size + b.abs()
     ok = allowed_of(mask, k, rows)
     ref = torch.where(ok, s / t, -INF)
-    # roundings before the last: rep, x / rep, freq, freq * c, pres, their sum, the difference, the sum with the bias, 1 / T,
-    # its product: 10, each at most u times `size` / T (times 1 + a few u: 12)
+    # roundings before the last, each at most u times `size` / T: rep, 1 / rep, its product, freq, freq * c, pres, their sum,
+    # the difference, the sum with the bias, T, 1 / T, its product: 12
     bound = ut * ref.abs() + 12 * u * size / t.abs() + tiny
     return ref.reshape(z.shape), torch.nan_to_num(bound, nan=0.0, posinf=0.0).reshape(z.shape)
 
@@ -198,7 +197,7 @@ def test_adjust_and_its_gradient(gpu, dt, rows, k):
         within(out, ref, bound)
         dz, db = cl.adjust_grad(g, z, **a)
         rz, rb = plain_adjust_grad(g, z, **a)
-        # 1 / T, its product, rep, its product or quotient: 4 roundings
+        # T, 1 / T, its product, rep, 1 / rep, its product: 6 roundings
         within(dz, rz, ut * rz.abs() + 6 * u * rz.abs() + tiny)
         if bias is None:
             assert db is None
@@ -255,6 +254,44 @@ def test_adjust_long_and_degenerate_histories(gpu):
     a = dict(history=torch.zeros(3, 0, dtype=torch.int64, device=gpu), presence=1.0, repetition=2.0)
     assert torch.equal(cl.adjust(z, **a), z)
     assert cl.adjust(z[:0], temperature=2.0).shape == (0, k)
+
+
+def test_adjust_counters_past_16_bits(gpu):
+    """A history longer than 32767 ids takes wider counters: one token 40000 times, some of them in the prompt."""
+    from distributions_amd import categorical_logits as cl
+
+    k, n = 5000, 40001
+    z = make((2, k), torch.float32, 3, gpu)
+    h = torch.full((2, n), 4097, dtype=torch.int32, device=gpu)
+    h[1, ::3] = 4096
+    a = dict(history=h, prompt_lengths=torch.tensor([1, 30000], device=gpu), frequency=0.25, presence=0.5, repetition=1.3)
+    ref, bound = plain_adjust(z, **a)
+    assert float(ref[0, 4097]) < -9999
+    within(cl.adjust(z, **a), ref, bound)
+    dz, _ = cl.adjust_grad(z, z, **a)
+    rz, _ = plain_adjust_grad(z, z, **a)
+    within(dz, rz, 8 * 2.0**-24 * rz.abs())
+
+
+@pytest.mark.parametrize("dt, mask, bias", [("f32", "bits", "shared"), ("bf16", "bool", "rows"), ("f16", "bits", None), ("f64", None, "rows")])
+def test_adjust_many_rows_of_several_chunks(gpu, dt, mask, bias):
+    """Rows dealt to the XCDs (their number no multiple of eight), several chunks a row, histories of several rounds."""
+    from distributions_amd import categorical_logits as cl
+
+    rows, k = 131, 20011
+    dtype, wide = DT[dt], torch.float64 if dt == "f64" else torch.float32
+    u, ut, tiny = steps(dtype)
+    z, g = make((rows, k), dtype, 1, gpu), make((rows, k), dtype, 2, gpu)
+    a = adjust_args(rows, k, 5, gpu, 1500, mask, bias, wide)
+    ref, bound = plain_adjust(z, **a)
+    within(cl.adjust(z, **a), ref, bound)
+    dz, db = cl.adjust_grad(g, z, **a)
+    rz, rb = plain_adjust_grad(g, z, **a)
+    within(dz, rz, ut * rz.abs() + 6 * u * rz.abs() + tiny)
+    if bias == "rows":
+        within(db, rb, 3 * u * rb.abs() + 2.0**-149)
+    elif bias:
+        within(db, rb.sum(0), 4 * u * rb.abs().sum(0) + 2.0**-149)
 
 
 def strided(z):
