@@ -44,7 +44,7 @@ def _bind():
         L.m355_logits_workspace_bytes.restype = _sz
         L.m355_logits_workspace_bytes.argtypes = [_i64, _i64, _i32]
         L.m355_logits_logpdf.restype = _i32
-        L.m355_logits_logpdf.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _vp, _sz, _vp]
+        L.m355_logits_logpdf.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _vp]
         L.m355_logits_sum_logpdf_grad.restype = _i32
         L.m355_logits_sum_logpdf_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, bp, _vp, _vp, _i64, _vp, _sz, _vp]
         _codes = {torch.float64: F64, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
@@ -368,12 +368,9 @@ def logpdf(x, logits):
         z, stride = _rows(t)
         xt, xcode = _observations(x, batch, torch, device)
         out = torch.empty(batch, dtype=_value_dtype(z, torch), device=device)
-        rows, code = z.shape[0], _codes[z.dtype]
-        if rows:
-            need = L.m355_logits_workspace_bytes(rows, k, code)
-            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            _lib.check(L.m355_logits_logpdf(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode, out.data_ptr(),
-                                            ws.data_ptr() if need else None, need, _stream(torch, device)))
+        if z.shape[0]:
+            _lib.check(L.m355_logits_logpdf(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, xt.data_ptr(), xcode,
+                                            out.data_ptr(), _stream(torch, device)))
     return out if isinstance(logits, torch.Tensor) or isinstance(x, torch.Tensor) else out.cpu().numpy()
 
 

@@ -918,15 +918,20 @@ template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStrea
   if (a.k <= kShort * 4) return launch_short<T, 4, GRAD>(a, s);
   if (a.k <= kShort * 16) return launch_short<T, 16, GRAD>(a, s);
   if (a.k <= kShort * 64) return launch_short<T, 64, GRAD>(a, s);
-  if constexpr (GRAD) {
-    constexpr bool wide = sizeof(typename T::store) == 8;
+  if constexpr (GRAD && sizeof(typename T::store) == 8) {  // float64 arithmetic takes registers from the row
     if (nv <= 64 * 4) launch_grad<T, 64, 4, 0, 4, false>(a, s);
-    else if (nv <= 256 * 4) launch_grad<T, 256, 4, 0, wide ? 4 : 8, false>(a, s);
+    else if (nv <= 256 * 4) launch_grad<T, 256, 4, 0, 4, false>(a, s);
     else if (nv <= 512 * 4) launch_grad<T, 512, 4, 0, 4, false>(a, s);
-    else if (nv <= 1024 * 4) launch_grad<T, 1024, 4, 0, wide ? 4 : 8, false>(a, s);
-    else if (nv <= 512 * 16 && !wide) launch_grad<T, 512, wide ? 8 : 16, 0, 4, false>(a, s);
-    else if (nv <= 512 * 32 && !wide) launch_grad<T, 512, wide ? 8 : 16, 0, 4, true>(a, s);
-    else launch_grad<T, 1024, wide ? 6 : 8, wide ? 6 : 4, 4, true>(a, s);
+    else if (nv <= 1024 * 4) launch_grad<T, 1024, 4, 0, 4, false>(a, s);
+    else launch_grad<T, 1024, 6, 6, 4, true>(a, s);
+  } else if constexpr (GRAD) {
+    if (nv <= 64 * 4) launch_grad<T, 64, 4, 0, 4, false>(a, s);
+    else if (nv <= 256 * 4) launch_grad<T, 256, 4, 0, 8, false>(a, s);
+    else if (nv <= 512 * 4) launch_grad<T, 512, 4, 0, 4, false>(a, s);
+    else if (nv <= 1024 * 4) launch_grad<T, 1024, 4, 0, 8, false>(a, s);
+    else if (nv <= 512 * 16) launch_grad<T, 512, 16, 0, 4, false>(a, s);
+    else if (nv <= 512 * 32) launch_grad<T, 512, 16, 0, 4, true>(a, s);
+    else launch_grad<T, 1024, 8, 4, 4, true>(a, s);
   } else {
     const dim3 grid((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid));
     if (nv <= 64 * 4) hipLaunchKernelGGL((k_logits_value<T, 64, 4>), grid, dim3(64), 0, s, a);
@@ -1102,15 +1107,13 @@ extern "C" size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype
 }
 
 extern "C" int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
-                                  const void* x, int x_dtype, void* out, void* workspace, size_t workspace_bytes,
-                                  void* stream) {
+                                  const void* x, int x_dtype, void* out, void* stream) {
   using namespace m355;
   DensityArgs a;
   const int rc = check_density(rows, k, dtype, logits, logits_stride, x, x_dtype, a);
   if (rc) return rc;
   if (rows == 0) return M355_OK;
-  if (!out || !workspace) return fail(M355_ERR_INVALID, "NULL pointer argument");
-  if (workspace_bytes < m355_logits_workspace_bytes(rows, k, dtype)) return fail(M355_ERR_WORKSPACE, "workspace too small");
+  if (!out) return fail(M355_ERR_INVALID, "NULL pointer argument");
   a.lp = out;
   by_dtype(dtype, [&](auto t) { return launch_density<decltype(t), false>(a, static_cast<hipStream_t>(stream)), 0; });
   return launched();

@@ -401,18 +401,18 @@ int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const void* g, i
 /*
  * out[r] = log-density of observation x[r] (M355_I64 / I32 / F64 / F32) under row r: z[x] - log sum exp(z).  -inf when x
  * is not an integer in [0, k) or when every logit of the row is -inf; NaN when the row holds NaN or +inf.
- * workspace: m355_logits_workspace_bytes bytes, 8-byte aligned, scratch; calls that may run concurrently need one each.
  */
-size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype);
 int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride, const void* x,
-                       int x_dtype, void* out, void* workspace, size_t workspace_bytes, void* stream);
+                       int x_dtype, void* out, void* stream);
 /*
  * total = sum_r w_r logpdf_r (added in float64, in a fixed order) and, unless dlogits is NULL, its gradient
  *     dlogits[r, v] = w_r ((v == x_r) - exp(z_v) / sum exp(z))   (dtype; 0 where x_r is no category or the whole row is -inf)
  * weights: operand over the row index (float64 / float32 array or scalar).  A row of weight 0 contributes 0 and gets
  * gradient 0, whatever it holds.  dlogits may be the logits themselves (same address and stride); any other overlap with
- * an input is undefined.
+ * an input is undefined.  workspace: m355_logits_workspace_bytes bytes, 8-byte aligned, scratch; calls that may run
+ * concurrently need one each.
  */
+size_t m355_logits_workspace_bytes(int64_t rows, int64_t k, int dtype);
 int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, const void* logits, int64_t logits_stride,
                                 const void* x, int x_dtype, const m355_operand* weights, void* total, void* dlogits,
                                 int64_t dlogits_stride, void* workspace, size_t workspace_bytes, void* stream);
