@@ -17,8 +17,10 @@ from ._lib import BF16, F16, F32, F64, I32, I64, LogitAdjust, Operand
 _L = _torch_module = None
 _codes = None  # torch dtype -> code of the types logits may have
 _x_codes = None  # ... observations may have
+_row_codes = None  # ... arguments per row may have
 _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 MASK_NONE, MASK_BYTES, MASK_BITS = 0, 1, 2
+_ONE, _ZERO = (0, 1.0, 1, 1, F64, 0), (0, 0.0, 1, 1, F64, 0)  # scalar operands
 # Calls of a few microseconds on the GPU come one after the other here, so the C structs are packed in one go: filling them
 # field by field took longer than the kernels.
 _OPERAND = "Qdqqii"
@@ -30,7 +32,7 @@ assert struct.calcsize("=QqqQQQqQqiiii" + 4 * _OPERAND) == ctypes.sizeof(LogitAd
 
 def _bind():
     """(torch, library), the argument types declared; raises without a GPU or the library."""
-    global _L, _torch_module, _codes, _x_codes
+    global _L, _torch_module, _codes, _x_codes, _row_codes
     if _L is None:
         torch = _check_torch()
         L = _lib.lib()
@@ -48,6 +50,7 @@ def _bind():
         L.m355_logits_sum_logpdf_grad.restype = _i32
         L.m355_logits_sum_logpdf_grad.argtypes = [_i64, _i64, _i32, _vp, _i64, _vp, _i32, bp, _vp, _vp, _i64, _vp, _sz, _vp]
         _codes = {torch.float64: F64, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        _row_codes = {torch.float64: F64, torch.float32: F32}
         _x_codes = {torch.int64: I64, torch.int32: I32, torch.float64: F64, torch.float32: F32}
         _torch_module, _L = torch, L
     return _torch_module, _L
@@ -92,18 +95,27 @@ def _rows(t):
     return t, t.stride(0)
 
 
+def _any_tensor(torch, first, *more):
+    return isinstance(first, torch.Tensor) or any(isinstance(a, torch.Tensor) for a in more)
+
+
 def _is_number(a):
     return type(a) is float or type(a) is int or (isinstance(a, (float, int, np.floating, np.integer)) and not isinstance(a, bool))
 
 
 def _row_operand(a, batch, torch, device, keep, what, positive=False):
     """The fields of an Operand from a per-row argument: a number, or an array that broadcasts to the rows' shape."""
-    if _is_number(a):
+    if isinstance(a, torch.Tensor):
+        code = _row_codes.get(a.dtype)
+        if code is not None and a.shape == batch and a.is_contiguous() and a.device == device:  # nothing to convert
+            keep.append(a)
+            return a.data_ptr(), 0.0, 1, a.numel() or 1, code, 0
+    elif _is_number(a):
         if positive and not a > 0:
             raise ValueError(f"{what} must be positive, got {a}")
         return 0, float(a), 1, 1, F64, 0
     t = _tensor(a, torch, device)
-    if t.dtype is not torch.float32 and t.dtype is not torch.float64:
+    if t.dtype not in _row_codes:
         t = t.to(torch.float64)
     if t.shape != batch:
         try:
@@ -116,7 +128,7 @@ def _row_operand(a, batch, torch, device, keep, what, positive=False):
             t = t.expand(batch)
     t = t.contiguous()
     keep.append(t)
-    return t.data_ptr(), 0.0, 1, max(t.numel(), 1), F32 if t.dtype is torch.float32 else F64, 0
+    return t.data_ptr(), 0.0, 1, t.numel() or 1, _row_codes[t.dtype], 0
 
 
 def _row_ints(a, batch, torch, device, keep, what):
@@ -124,6 +136,9 @@ def _row_ints(a, batch, torch, device, keep, what):
     if a is None:
         return 0
     t = _tensor(a, torch, device)
+    if t.dtype is torch.int64 and t.shape == batch and t.is_contiguous():
+        keep.append(t)
+        return t.data_ptr()
     if t.dtype is not torch.int64:
         if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
             raise TypeError(f"{what}: integers, got {t.dtype}")
@@ -163,18 +178,19 @@ def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths
     """The C struct of an adjustment (packed), the tensors it points to, the bias as given (tensor or None) and whether all
     rows share it."""
     keep = []
-    rep = _row_operand(repetition, batch, torch, device, keep, "repetition", positive=True)
-    pres = _row_operand(presence, batch, torch, device, keep, "presence")
-    freq = _row_operand(frequency, batch, torch, device, keep, "frequency")
     temp = _row_operand(temperature, batch, torch, device, keep, "temperature", positive=True)
     hist = hist_len = hist_stride = hist_code = lens = prompts = 0
     if history is None:
         if lengths is not None or prompt_lengths is not None:
             raise ValueError("lengths and prompt_lengths belong to a history")
-        for what, a, neutral in (("repetition", repetition, 1), ("presence", presence, 0), ("frequency", frequency, 0)):
-            if not (_is_number(a) and a == neutral):
+        for what, a, neutral in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
+            if a is not neutral and not (_is_number(a) and a == neutral):
                 raise ValueError(f"{what} needs a history")
+        rep, pres, freq = _ONE, _ZERO, _ZERO
     else:
+        rep = _row_operand(repetition, batch, torch, device, keep, "repetition", positive=True)
+        pres = _row_operand(presence, batch, torch, device, keep, "presence")
+        freq = _row_operand(frequency, batch, torch, device, keep, "frequency")
         h = _tensor(history, torch, device)
         if h.dtype is not torch.int64 and h.dtype is not torch.int32:
             if h.is_floating_point() or h.is_complex() or h.dtype is torch.bool:
@@ -245,19 +261,22 @@ def _out_rows(out, z, inputs, torch):
     return o, o.stride(0)
 
 
-class _on:
-    """The device as HIP's current one for the launch; no switch where it is already."""
-
-    def __init__(self, torch, device):
-        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+class _Here:
+    """No switch of devices: a context that does nothing."""
 
     def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
+        pass
 
     def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
+        pass
+
+
+_here = _Here()
+
+
+def _on(torch, device):
+    """The device as HIP's current one for the launch; no switch where it is already."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def adjust(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask, out):
@@ -281,7 +300,7 @@ def adjust(logits, history, lengths, prompt_lengths, repetition, presence, frequ
             _lib.check(L.m355_logits_adjust(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, d, o.data_ptr(), ostride,
                                             _stream(torch, device)))
         del keep
-    return res if out is not None or any(isinstance(a, torch.Tensor) for a in args) else res.cpu().numpy()
+    return res if out is not None or _any_tensor(torch, *args) else res.cpu().numpy()
 
 
 def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask):
@@ -318,7 +337,7 @@ def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presenc
             if b is not bias and getattr(bias, "dtype", None) is not None:  # it was converted: back to its own type
                 db = db.to(_float_type(bias, db.dtype, torch))
         del keep
-    if any(isinstance(a, torch.Tensor) for a in args):
+    if _any_tensor(torch, logits, *args):
         return dz, db
     return dz.cpu().numpy(), None if db is None else db.cpu().numpy()
 
@@ -343,6 +362,9 @@ def _sum_to(t, shape):
 
 def _observations(x, batch, torch, device):
     t = _tensor(x, torch, device)
+    code = _x_codes.get(t.dtype)
+    if code is not None and t.shape == batch and t.is_contiguous():
+        return t, code
     if t.dtype not in _x_codes:
         if t.is_complex():
             raise TypeError("observations are integers or floats")
@@ -402,6 +424,6 @@ def sum_logpdf(x, logits, weights, grad, out=None):
                                                  o.data_ptr() if grad and rows else None, ostride, ws.data_ptr(), need,
                                                  _stream(torch, device)))
         del keep
-    if out is not None or any(isinstance(a, torch.Tensor) for a in args):
+    if out is not None or _any_tensor(torch, logits, *args):
         return total, dz
     return float(total.item()), None if dz is None else dz.cpu().numpy()

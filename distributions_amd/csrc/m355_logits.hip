@@ -161,7 +161,9 @@ template <class C> struct Penalties {
 
 // One workgroup per (row, chunk): everything the chunk needs from memory is fetched first, then, with a history (CNT: the
 // type of its counters, or void), the ids that fall into the chunk are counted in LDS, then the pieces are worked off.  The
-// k % kPer last categories of a row belong to the first threads of its last chunk.
+// k % kPer last categories of a row belong to the first threads of its last chunk.  Without a history bound by HBM (1024 x
+// 65537 float32: 94 us, 5.7 TB/s, rows at odd addresses); with one by the chain ids -> counters -> barrier -> stores: 256 x
+// 100003 float32 with 4001 ids 48 us (4.4 TB/s), 64 x 131072 bf16 with 2048 ids 12.7 us.
 template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD>
 __global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustArgs a, const AdjustGrid grid) {
   typedef typename T::comp comp;
@@ -342,7 +344,7 @@ template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_l
 // Gradient of a bias that all rows share.  A workgroup of G groups of CT threads takes CT * kPer columns and a block of rows;
 // a thread owns kPer columns and every G-th row of the block, so that the column sums stay in its registers (float64) and
 // kSumRows rows are in flight; the groups are joined in LDS, the row blocks by k_logits_cols_final, all in a fixed order.
-// Without a history the gradient of the logits is written on the way.
+// Without a history the gradient of the logits is written on the way.  4096 x 32768 bf16 with a mask: 130 us, 5.2 TB/s.
 constexpr int kSumThreads = 512, kSumRows = 4;
 
 template <class T, int CT, bool WRITE>
@@ -524,10 +526,13 @@ template <class T> M355_DEV void repack(raw_t<T>& r) {
   r.x = v.x, r.y = v.y, r.z = v.z, r.w = v.w;
 }
 
-// Value and gradient, one row per workgroup.  The row is read once: its first NR * THREADS 16-byte pieces wait in registers,
+// Value and gradient, one row per workgroup: z[x] - m - log s and w ([v = x] - exp(z - m) / s), m the row's maximum, s its sum
+// of exp(z - m).  The row is read once: its first NR * THREADS 16-byte pieces wait in registers,
 // the next NL * THREADS in LDS, while maximum and sum are formed; what does not fit there is summed as it passes and read
 // again for the gradient.  The k % kPer last elements belong to the first threads, one each.  In place (grad == z): a row is
-// read before it is written, but for the pieces that are read again, which the same thread reads and writes.
+// read before it is written, but for the pieces that are read again, which the same thread reads and writes.  Bound by HBM and
+// by how far the phases (load, sum, store) of the workgroups of a CU overlap: 4096 x 131072 bf16, an eighth of the rows padding,
+// 403 us (5.0 TB/s of what has to move, where a copy reaches 6.5), 1500 x 100003 float32 243 us.
 template <class T, int THREADS, int NR, int NL, int WAVES, bool REST>
 __global__ __launch_bounds__(THREADS, WAVES) void k_logits_grad(const DensityArgs a) {
   typedef typename T::comp comp;
@@ -737,7 +742,8 @@ template <class T, int G, bool GRAD> __global__ __launch_bounds__(256) void k_lo
   }
 }
 
-// Value only: one row per workgroup, tiles of NR 16-byte loads per thread with a running maximum and sum.
+// Value only: one row per workgroup, tiles of NR 16-byte loads per thread with a running maximum and sum.  Bound by HBM:
+// 8192 x 32768 float16 in 83 us, 6.5 TB/s.
 template <class T, int THREADS, int NR>
 __global__ __launch_bounds__(THREADS) void k_logits_value(const DensityArgs a) {
   constexpr int N = kPer<T>;
@@ -847,8 +853,8 @@ template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD
 
 template <class T, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   // Four pieces per thread hide the latencies of a chunk behind each other; where that gives too few workgroups for 256
-  // CUs, one piece each (1 x 32768 bf16: 4.9 against 7.1 us).  512 threads halve how often a history is scanned, and cost
-  // more than they save (512 x 131072 bf16, 500 ids: 71 against 60 us; 256 x 65536, 8000 ids: 36.8 against 37.6 us).
+  // CUs, one piece each (1 x 32768 bf16, 300 ids: 4.4 against 5.4 us).  512 threads halve how often a history is scanned, and
+  // cost more than they save (512 x 131072 bf16, 500 ids: 77 against 71 us; 256 x 65536, 8000 ids: 41.0 against 42.3 us).
   const bool few = a.rows * (a.k / kPer<T>) < 256ll * 1024;
   if (!a.history && a.k / kPer<T> < 256) {  // a workgroup per row would be half empty
     const int pieces = (int)((a.k + kPer<T> - 1) / kPer<T>);
