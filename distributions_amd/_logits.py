@@ -350,14 +350,30 @@ def _float_type(a, otherwise, torch):
 
 
 def _sum_to(t, shape):
-    """The gradient of an operand that was broadcast along some of the rows' axes only."""
+    """The gradient of an operand that was broadcast along some of the rows' axes only: summed along those by halves, in a
+    fixed order.  (Additions of slices: a library sum over many blocks clears memory in a way that a captured graph does not
+    repeat.)"""
     if tuple(t.shape) == tuple(shape):
         return t
     lead = t.dim() - len(shape)
     axes = tuple(range(lead)) + tuple(lead + i for i, n in enumerate(shape) if n == 1 and t.shape[lead + i] != 1)
-    acc = t.dtype if t.element_size() >= 4 else None
-    s = t.sum(dim=axes, keepdim=True) if acc is not None else t.float().sum(dim=axes, keepdim=True).to(t.dtype)
-    return s.reshape(shape)
+    s = t if t.element_size() >= 4 else t.float()
+    for axis in axes:
+        if s.shape[axis] == 0:
+            s = s.new_zeros([1 if i == axis else n for i, n in enumerate(s.shape)])
+        while s.shape[axis] > 1:
+            n = s.shape[axis]
+            half = (n + 1) // 2
+            low, high = s.narrow(axis, 0, half), s.narrow(axis, half, n - half)
+            s = low + high if n == 2 * half else _cat_last(low, high, axis)
+    return s.to(t.dtype).reshape(shape)
+
+
+def _cat_last(low, high, axis):
+    """low + high with one slice of low left over at the end."""
+    res = low.clone()
+    res.narrow(axis, 0, high.shape[axis]).add_(high)
+    return res
 
 
 def _observations(x, batch, torch, device):

@@ -625,6 +625,58 @@ def test_step_against_autograd(gpu, dt):
     assert float((db.cpu().double() - br.grad * f).norm()) <= tol * 0.5
 
 
+def test_bias_shared_by_some_axes(gpu):
+    """A bias that is broadcast along some of the rows' axes: its gradient, eager and captured."""
+    from distributions_amd import categorical_logits as cl
+
+    for shape, bshape in (((3, 7, 50), (3, 1, 50)), ((3, 7, 50), (7, 50)), ((2, 5, 3, 9), (2, 1, 3, 9)), ((2, 5, 3, 9), (5, 1, 9))):
+        g = make(shape, torch.float32, 1, gpu)
+        z = make(shape, torch.float32, 2, gpu)
+        bias = make(bshape, torch.float32, 3, gpu)
+        full = (1,) * (len(shape) - len(bshape)) + bshape
+        axes = [i for i, (m, n) in enumerate(zip(full, shape)) if m != n]
+        ref = g.cpu().double().sum(axes, keepdim=True).reshape(bshape)
+        size = g.cpu().double().abs().sum(axes, keepdim=True).reshape(bshape)
+        _, db = cl.adjust_grad(g, z, bias=bias)
+        within(db, ref, 8 * 2.0**-24 * size)  # T and its quotient 1; at most 4 + 2 additions by halves
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            cl.adjust_grad(g, z, bias=bias)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _, captured = cl.adjust_grad(g, z, bias=bias)
+        for i in range(3):
+            g.copy_(make(shape, torch.float32, 10 + i, gpu))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(captured, cl.adjust_grad(g, z, bias=bias)[1])
+
+
+def test_two_streams_at_once(gpu):
+    """Steps of two problems that are under way together on two streams give what each gives alone."""
+    work, want = [], []
+    for i, (rows, k) in enumerate(((300, 4001), (17, 60000))):
+        z = make((rows, k), torch.bfloat16, 70 + i, gpu)
+        a = adjust_args(rows, k, 72 + i, gpu, 300, "bool", "shared")
+        a["mask"][-1] = True
+        x = torch.arange(rows, device=gpu)
+        a["mask"][torch.arange(rows, device=gpu), x] = True
+        work.append((z, x, torch.ones(rows, device=gpu), a, 0.3))
+        want.append(step(*work[-1]))
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*work[i]))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(p, q) for r in runs for p, q in zip(w, r))
+
+
 def test_streams_and_captured_graphs(gpu):
     """A step on another stream, and two captured graphs of it replayed in turn with eager work in between."""
     rows, k = 33, 5003
