@@ -164,8 +164,8 @@ template <class C> struct Penalties {
 // k % kPer last categories of a row belong to the first threads of its last chunk.  Without a history bound by HBM (1024 x
 // 65537 float32: 94 us, 5.7 TB/s, rows at odd addresses); with one by the chain ids -> counters -> barrier -> stores: 256 x
 // 100003 float32 with 4001 ids 48 us (4.4 TB/s), 64 x 131072 bf16 with 2048 ids 12.7 us.
-template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD>
-__global__ __launch_bounds__(THREADS, WAVES) void k_logits_adjust(const AdjustArgs a, const AdjustGrid grid) {
+template <class T, int THREADS, int VPT, class CNT, class B, bool BWD>
+__global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a, const AdjustGrid grid) {
   typedef typename T::comp comp;
   typedef typename T::store store;
   constexpr int N = kPer<T>;
@@ -838,7 +838,7 @@ __global__ __launch_bounds__(1024) void k_logits_total(const C* __restrict__ lp,
 // ---------------------------------------------------------------------------------------------- launches
 constexpr long long kMaxGrid = 1ll << 21;  // workgroups (the launch counts threads in 32 bits); kernels walk on from there
 
-template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+template <class T, int THREADS, int VPT, class CNT, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   const long long nv = a.k / kPer<T>;
   AdjustGrid g;
   g.chunks = (int)((nv + THREADS * VPT - 1) / (THREADS * VPT));
@@ -847,7 +847,7 @@ template <class T, int THREADS, int VPT, int WAVES, class CNT, class B, bool BWD
   if (g.per > 0) g.chunks = (int)((nv + g.per - 1) / g.per);  // and none that is empty
   g.rows_by_xcd = a.rows >= 64;
   g.items = (g.rows_by_xcd ? (a.rows + 7) / 8 * 8 : a.rows) * g.chunks;
-  hipLaunchKernelGGL((k_logits_adjust<T, THREADS, VPT, WAVES, CNT, B, BWD>), dim3((unsigned)(g.items < kMaxGrid ? g.items : kMaxGrid)),
+  hipLaunchKernelGGL((k_logits_adjust<T, THREADS, VPT, CNT, B, BWD>), dim3((unsigned)(g.items < kMaxGrid ? g.items : kMaxGrid)),
                      dim3(THREADS), 0, s, a, g);
 }
 
@@ -863,10 +863,10 @@ template <class T, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hi
                        s, a, pieces);
     return;
   }
-  if (!a.history) few ? launch_adjust<T, 256, 1, 8, void, B, BWD>(a, s) : launch_adjust<T, 256, 4, 4, void, B, BWD>(a, s);
-  else if (a.history_len > 32767) launch_adjust<T, 256, 4, 4, unsigned, B, BWD>(a, s);
-  else if (few) launch_adjust<T, 256, 1, 8, unsigned short, B, BWD>(a, s);
-  else launch_adjust<T, 256, 4, 4, unsigned short, B, BWD>(a, s);
+  if (!a.history) few ? launch_adjust<T, 256, 1, void, B, BWD>(a, s) : launch_adjust<T, 256, 4, void, B, BWD>(a, s);
+  else if (a.history_len > 32767) launch_adjust<T, 256, 4, unsigned, B, BWD>(a, s);
+  else if (few) launch_adjust<T, 256, 1, unsigned short, B, BWD>(a, s);
+  else launch_adjust<T, 256, 4, unsigned short, B, BWD>(a, s);
 }
 
 // forward: with the bias, if there is one; gradient: with a bias' gradient that goes out per element
@@ -909,16 +909,17 @@ template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launc
                      dim3((unsigned)(a.rows < kMaxGrid ? a.rows : kMaxGrid)), dim3(THREADS), 0, s, a);
 }
 
-// Lanes per short row; pieces per thread and threads per workgroup by the length of longer ones.  Measured for bf16 (r + w, 5.1-5.7 TB/s; a copy reaches
-// 6.4): four pieces per thread beat eight of half the threads while a row fits 1024 threads (8192 x 32768: 194 against
-// 208 us), then two workgroups of 512 threads a CU beat one of 1024 (4096 x 131072: 415 against 437-450 us) although
-// they read half of the row twice, from the Infinity Cache; rows over 256 KiB take one workgroup a CU again (float32,
-// 1500 x 100003: 256 against 277 us), because the rows of 512 workgroups no longer fit that cache.
 template <class T, int G, bool GRAD> void launch_short(const DensityArgs& a, hipStream_t s) {
   const long long want = (a.rows * G + 255) / 256;
   hipLaunchKernelGGL((k_logits_short<T, G, GRAD>), dim3((unsigned)(want < kMaxGrid ? want : kMaxGrid)), dim3(256), 0, s, a);
 }
 
+// Lanes per short row; pieces per thread and threads per workgroup by the length of longer ones.  Gradient, measured for
+// bf16 (reads and writes at 5.0-5.7 TB/s; a copy reaches 6.5): four pieces per thread beat eight of half the threads while a
+// row fits 1024 threads (8192 x 32768: 194 against 208 us), then two workgroups of 512 threads a CU beat one of 1024 (4096 x
+// 131072: 415 against 437-450 us) although they read half of the row twice; rows over 256 KiB take one workgroup a CU again
+// (float32, 1500 x 100003: 256 against 277 us), as less of them is read twice.  Value: enough rows fill the chip with 256
+// threads each, few rows take 1024 (8 x 50021 float32: 7 against 17 us).
 template <class T, bool GRAD> void launch_density(const DensityArgs& a, hipStream_t s) {
   const long long nv = a.k / kPer<T>;
   if (a.k <= kShort * 4) return launch_short<T, 4, GRAD>(a, s);

@@ -618,7 +618,7 @@ def test_step_against_autograd(gpu, dt):
     n = torch.sqrt(zr.grad.square().sum() + br.grad.square().sum())
     # logits between -20 and 20 are rounded once on the way (20 ut each), gradients twice: relative to the whole
     tol = 40 * ut + 4000 * u
-    assert abs(float(total) - float(ref)) <= tol * rows
+    assert abs(float(total) - float(ref.detach())) <= tol * rows
     assert abs(float(norm) - float(n)) <= tol * float(n)
     f = 0.5 / float(n)
     assert float((dz.cpu().double() - zr.grad * f).norm()) <= tol * 0.5
