@@ -55,18 +55,22 @@ class _List:
             raise TypeError("a list of gradients is expected, got one array")
         self.grads = grads = list(grads)
         self.places = range(len(grads))
-        if any(g is None for g in grads):
+        plain = {type(g) for g in grads} <= {torch.Tensor}  # tensors only: nothing to sort out
+        tensors = grads
+        if not plain:
             self.places = [i for i, g in enumerate(grads) if g is not None]
-        tensors = grads if len(self.places) == len(grads) else [grads[i] for i in self.places]
-        devices = {g.device for g in tensors if isinstance(g, torch.Tensor)}
+            tensors = [grads[i] for i in self.places]
+        devices = {g.device for g in tensors if plain or isinstance(g, torch.Tensor)}
         self.want_torch = bool(devices)
         if len(devices) > 1:
             raise ValueError("gradients on several devices")
         self.device = devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
         if self.device.type != "cuda":
             raise ValueError("gradients are CUDA tensors (or NumPy arrays)")
-        self.tensors = [g if isinstance(g, torch.Tensor) else
-                        torch.from_numpy(np.array(np.asarray(g), order="C", copy=True)).to(self.device) for g in tensors]
+        if not plain:
+            tensors = [g if isinstance(g, torch.Tensor) else
+                       torch.from_numpy(np.array(np.asarray(g), order="C", copy=True)).to(self.device) for g in tensors]
+        self.tensors = tensors
         self.dtypes = [g.dtype for g in self.tensors]
         kinds = set(self.dtypes)
         for dt in kinds:
