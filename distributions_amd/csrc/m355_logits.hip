@@ -893,6 +893,10 @@ template <class T> ColumnGrid column_grid(long long rows, long long k) {
   return g;
 }
 
+template <class T> void launch_cols_final(const AdjustArgs& a, const double* ws, int row_blocks, void* dbias, hipStream_t s) {
+  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + 63) / 64)), dim3(256), 0, s, ws, a.k, row_blocks, dbias,
+                     a.bias_dtype);
+}
 template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, double* ws, hipStream_t s) {
   const ColumnGrid g = column_grid<T>(a.rows, a.k);
   const dim3 grid((unsigned)((long long)g.chunks * g.row_blocks)), block(kSumThreads);
@@ -900,8 +904,7 @@ template <class T> void launch_adjust_cols(const AdjustArgs& a, void* dbias, dou
   if (g.ct == 8) a.dst ? launch(k_logits_adjust_cols<T, 8, true>) : launch(k_logits_adjust_cols<T, 8, false>);
   else if (g.ct == 32) a.dst ? launch(k_logits_adjust_cols<T, 32, true>) : launch(k_logits_adjust_cols<T, 32, false>);
   else a.dst ? launch(k_logits_adjust_cols<T, 128, true>) : launch(k_logits_adjust_cols<T, 128, false>);
-  hipLaunchKernelGGL((k_logits_cols_final<T>), dim3((unsigned)((a.k + 63) / 64)), dim3(256), 0, s, ws, a.k, g.row_blocks,
-                     dbias, a.bias_dtype);
+  launch_cols_final<T>(a, ws, g.row_blocks, dbias, s);
 }
 
 template <class T, int THREADS, int NR, int NL, int WAVES, bool REST> void launch_grad(const DensityArgs& a, hipStream_t s) {
@@ -1082,9 +1085,14 @@ extern "C" int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const
   if (dbias && !a.bias) return fail(M355_ERR_INVALID, "dbias without a bias");
   const bool shared = dbias && a.bias_ld == 0;
   if (shared && k > (INT64_C(1) << 28)) return fail(M355_ERR_INVALID, "gradient of a shared bias: at most 2^28 categories");
-  if (rows == 0 && !shared) return M355_OK;
-  if ((rows && (!g || (dlogits && a.history && !logits)))) return fail(M355_ERR_INVALID, "NULL pointer argument");
-  if (shared && rows && (!workspace || workspace_bytes < m355_logits_adjust_grad_workspace_bytes(rows, k, dtype)))
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) {  // no row blocks: a workspace is neither asked for nor read, and the sums are 0
+    if (!shared) return M355_OK;
+    by_dtype(dtype, [&](auto t) { return launch_cols_final<decltype(t)>(a, nullptr, 0, dbias, s), 0; });
+    return launched();
+  }
+  if (!g || (dlogits && a.history && !logits)) return fail(M355_ERR_INVALID, "NULL pointer argument");
+  if (shared && (!workspace || workspace_bytes < m355_logits_adjust_grad_workspace_bytes(rows, k, dtype)))
     return fail(M355_ERR_WORKSPACE, "workspace too small");
   a.src = g;
   a.src_ld = g_stride;
@@ -1093,7 +1101,6 @@ extern "C" int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const
   a.dst = dlogits;
   a.dst_ld = k;
   a.dbias = shared ? nullptr : dbias;
-  hipStream_t s = static_cast<hipStream_t>(stream);
   by_dtype(dtype, [&](auto t) {
     typedef decltype(t) T;
     if (shared) {

@@ -392,7 +392,8 @@ int m355_logits_adjust(int64_t rows, int64_t k, int dtype, const void* logits, i
  *     dbias   = allowed ? g / temperature : 0, per element (bias_stride != 0: rows x k contiguous values of bias_dtype)
  *               or summed over the rows in a fixed order, in float64 (bias_stride == 0: k values, k <= 2^28)
  * dlogits (rows x k contiguous) or dbias may be NULL: not wanted.  logits is read only with a history.  workspace:
- * m355_logits_adjust_grad_workspace_bytes bytes, 8-byte aligned, needed with dbias and bias_stride 0; scratch.
+ * m355_logits_adjust_grad_workspace_bytes bytes, 8-byte aligned, needed with dbias and bias_stride 0; scratch.  With no rows
+ * that is none, and the dbias that all rows share becomes 0.
  */
 size_t m355_logits_adjust_grad_workspace_bytes(int64_t rows, int64_t k, int dtype);
 int m355_logits_adjust_grad(int64_t rows, int64_t k, int dtype, const void* g, int64_t g_stride, const void* logits,

@@ -515,6 +515,28 @@ def test_weights_below_the_arithmetic(gpu, k):
     within(g, grad, b_g)
 
 
+@pytest.mark.parametrize("dt", DT)
+def test_shared_bias_gradient_of_no_rows(gpu, dt):
+    """Through the C-ABI, with the workspace it asks for (none): the sums over no rows are 0, and nothing else is written."""
+    from distributions_amd import _lib, _logits
+    from distributions_amd import categorical_logits as cl
+
+    dtype, k = DT[dt], 1003
+    torch_, L = _logits._bind()
+    for history in (None, torch.zeros(0, 5, dtype=torch.int64, device=gpu)):
+        buf = torch.full((k + 40,), 7.0, dtype=dtype, device=gpu)
+        bias = torch.zeros(k, dtype=dtype, device=gpu)
+        d, keep, *_ = _logits._adjustment((0,), k, dtype, torch_, bias.device, history, None, None, 1.0, 0.0, 0.0, bias, 1.0, None)
+        code = _logits._codes[dtype]
+        assert L.m355_logits_adjust_grad_workspace_bytes(0, k, code) == 0
+        _lib.check(L.m355_logits_adjust_grad(0, k, code, None, k, None, k, d, None, buf[20:].data_ptr(), None, 0,
+                                             _logits._stream(torch_, bias.device)))
+        assert bool((buf[20 : 20 + k] == 0).all()) and bool((buf[:20] == 7).all()) and bool((buf[20 + k :] == 7).all())
+        empty = torch.empty(0, k, dtype=dtype, device=gpu)
+        dz, db = cl.adjust_grad(empty, empty, history=history, bias=bias)
+        assert dz.shape == (0, k) and db.shape == (k,) and bool((db == 0).all())
+
+
 def test_bias_of_another_type(gpu):
     from distributions_amd import categorical_logits as cl
 
