@@ -174,10 +174,10 @@ def _wide_rows(t, batch, width, keep, what):
 
 
 def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths, repetition, presence, frequency, bias,
-                temperature, mask):
-    """The C struct of an adjustment (packed), the tensors it points to, the bias as given (tensor or None) and whether all
-    rows share it."""
-    keep = []
+                temperature, mask, grad=False):
+    """The C struct of an adjustment (packed; grad: of its gradient), the tensors it points to, the bias as given (tensor or
+    None) and whether all rows share it."""
+    keep, shared = [], False
     temp = _row_operand(temperature, batch, torch, device, keep, "temperature", positive=True)
     hist = hist_len = hist_stride = hist_code = lens = prompts = 0
     if history is None:
@@ -212,6 +212,9 @@ def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths
         if b.dtype is not dtype and not (b.dtype is torch.float32 and dtype is not torch.float64):
             given = b = b.to(torch.float64 if dtype is torch.float64 else torch.float32)
         b, bias_stride = _wide_rows(b, batch, k, keep, "bias")
+        shared = prod(given.shape[:-1]) == 1
+        if grad and not shared:  # an expanded view has stride 0 too, but a gradient per row; the values are not read there
+            bias_stride = k
         bias_ptr, bias_code = b.data_ptr(), _codes[b.dtype]
     mask_ptr = mask_stride = mask_kind = 0
     if mask is not None:
@@ -226,7 +229,7 @@ def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths
         mask_ptr = m.data_ptr()
     packed = _pack_adjust(hist, hist_len, hist_stride, lens, prompts, bias_ptr, bias_stride, mask_ptr, mask_stride, hist_code,
                           bias_code, mask_kind, 0, *rep, *pres, *freq, *temp)
-    return packed, keep, given, bias_stride == 0
+    return packed, keep, given, shared
 
 
 def _span(t):
@@ -317,7 +320,7 @@ def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presenc
             raise ValueError(f"g has shape {tuple(gt.shape)}, the logits {tuple(shape)}")
         gz, gstride = _rows(gt.to(z.dtype))
         d, keep, b, shared = _adjustment(shape[:-1], k, z.dtype, torch, device, history, lengths, prompt_lengths, repetition,
-                                         presence, frequency, bias, temperature, mask)
+                                         presence, frequency, bias, temperature, mask, grad=True)
         rows, code = z.shape[0], _codes[z.dtype]
         dz = torch.empty(shape, dtype=z.dtype, device=device)
         db, ws, need = None, None, 0

@@ -537,6 +537,29 @@ def test_shared_bias_gradient_of_no_rows(gpu, dt):
         assert dz.shape == (0, k) and db.shape == (k,) and bool((db == 0).all())
 
 
+@pytest.mark.parametrize("dt", DT)
+def test_expanded_bias(gpu, dt):
+    """A bias that is an expanded view gets a gradient per row, as a contiguous one of the same shape does."""
+    from distributions_amd import categorical_logits as cl
+
+    k, wide = 1003, torch.float64 if dt == "f64" else torch.float32
+    for batch, bshape in (((4,), (4, k)), ((2, 7), (2, 7, k)), ((2, 7), (2, 1, k)), ((2, 7), (7, k)), ((1,), (1, k)), ((3, 5), (1, 5, k))):
+        z, g = make((*batch, k), DT[dt], 1, gpu), make((*batch, k), DT[dt], 2, gpu)
+        for bdt in {DT[dt], wide}:
+            base = make((k,), bdt, 3, gpu)
+            bias = base.expand(bshape)
+            full = bias.contiguous()
+            assert torch.equal(cl.adjust(z, bias=bias), cl.adjust(z, bias=full))
+            dz, db = cl.adjust_grad(g, z, bias=bias, temperature=0.7)
+            dz2, db2 = cl.adjust_grad(g, z, bias=full, temperature=0.7)
+            assert torch.equal(dz, dz2) and db.shape == bshape and db.dtype == bdt and torch.equal(db, db2)
+            if len(batch) == 1 or bshape == (*batch, k):
+                u, ut, tiny = steps(bdt)
+                ref = g.cpu().double() / 0.7
+                # T, 1 / T, its product in the arithmetic of the logits, then the bias' own type
+                within(db, ref.reshape(bshape), (ut + 3 * steps(DT[dt])[0]) * ref.abs() + tiny)
+
+
 def test_bias_of_another_type(gpu):
     from distributions_amd import categorical_logits as cl
 

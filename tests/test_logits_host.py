@@ -134,6 +134,21 @@ def test_rows_and_layouts():
     assert _gradnorm.dense(torch.zeros(0, 4)) and _gradnorm.dense(torch.zeros(()))
 
 
+def test_expanded_bias_is_not_shared(L):
+    """Whether rows share a bias is a matter of its shape: an expanded view has row stride 0 and a gradient per row."""
+    codes = dict(zip((torch.float64, torch.float32, torch.float16, torch.bfloat16), (F64, F32, F16, BF16)))
+    one = torch.zeros(10)
+    for batch, bias, shared in (((4,), one.expand(4, 10), False), ((2, 7), one.expand(2, 1, 10), False), ((2, 7), one.expand(7, 10), False),
+                                ((2, 7), one.expand(2, 7, 10), False), ((4,), one, True), ((4,), one[None], True),
+                                ((2, 7), one[None, None], True), ((1,), one.expand(1, 10), True)):
+        assert _logits._codes == codes
+        for grad in (False, True):
+            packed, keep, given, got = _logits._adjustment(batch, 10, torch.float32, torch, torch.device("cpu"), None, None, None, 1.0, 0.0,
+                                                           0.0, bias, 1.0, None, grad=grad)
+            stride = LogitAdjust.from_buffer_copy(packed).bias_stride
+            assert given is bias and got is shared and (stride != 0) == (grad and not shared), (batch, bias.shape, grad)
+
+
 def test_sharded_clip_adds_the_ranks(monkeypatch):
     """The sum of squares of this rank is what is all-reduced, and the reduced one is what scales."""
     from distributions_amd import sharded
