@@ -173,6 +173,11 @@ def _wide_rows(t, batch, width, keep, what):
     return t, stride
 
 
+def _partly(bias, shared, batch):
+    """Whether a bias is shared along some of the rows' axes: its gradient comes per element and is summed by _sum_to."""
+    return not shared and bias.shape[:-1] != batch
+
+
 def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths, repetition, presence, frequency, bias,
                 temperature, mask, grad=False):
     """The C struct of an adjustment (packed; grad: of its gradient), the tensors it points to, the bias as given (tensor or
@@ -216,6 +221,8 @@ def _adjustment(batch, k, dtype, torch, device, history, lengths, prompt_lengths
         if grad and not shared:  # an expanded view has stride 0 too, but a gradient per row; the values are not read there
             bias_stride = k
         bias_ptr, bias_code = b.data_ptr(), _codes[b.dtype]
+        if grad and _partly(given, shared, batch):  # what is summed afterwards is not rounded to 16 bits before
+            bias_code = _codes[_value_dtype(dtype, torch)]
     mask_ptr = mask_stride = mask_kind = 0
     if mask is not None:
         m = _tensor(mask, torch, device)
@@ -325,7 +332,8 @@ def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presenc
         dz = torch.empty(shape, dtype=z.dtype, device=device)
         db, ws, need = None, None, 0
         if b is not None:
-            db = torch.empty(k if shared else shape, dtype=b.dtype, device=device)
+            partly = _partly(b, shared, shape[:-1])
+            db = torch.empty(k if shared else shape, dtype=_value_dtype(z.dtype, torch) if partly else b.dtype, device=device)
             if shared:
                 need = L.m355_logits_adjust_grad_workspace_bytes(rows, k, code)
                 ws = torch.empty(need, dtype=torch.uint8, device=device)
@@ -336,9 +344,10 @@ def adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presenc
                                                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
                                                  need, _stream(torch, device)))
         if b is not None:
-            db = db.reshape(b.shape) if shared else _sum_to(db, b.shape)
+            back = b.dtype
             if b is not bias and getattr(bias, "dtype", None) is not None:  # it was converted: back to its own type
-                db = db.to(_float_type(bias, db.dtype, torch))
+                back = _float_type(bias, back, torch)
+            db = _sum_to(db, b.shape).to(back) if partly else db.reshape(b.shape).to(back)
         del keep
     if _any_tensor(torch, logits, *args):
         return dz, db
@@ -353,30 +362,21 @@ def _float_type(a, otherwise, torch):
 
 
 def _sum_to(t, shape):
-    """The gradient of an operand that was broadcast along some of the rows' axes only: summed along those by halves, in a
-    fixed order.  (Additions of slices: a library sum over many blocks clears memory in a way that a captured graph does not
-    repeat.)"""
-    if tuple(t.shape) == tuple(shape):
-        return t
+    """The gradient of an operand that was broadcast along some of the rows' axes only: summed along those by halves, in
+    float64 and a fixed order.  (Additions of slices: a library sum over many blocks clears memory in a way that a captured
+    graph does not repeat.)"""
     lead = t.dim() - len(shape)
     axes = tuple(range(lead)) + tuple(lead + i for i, n in enumerate(shape) if n == 1 and t.shape[lead + i] != 1)
-    s = t if t.element_size() >= 4 else t.float()
     for axis in axes:
-        if s.shape[axis] == 0:
-            s = s.new_zeros([1 if i == axis else n for i, n in enumerate(s.shape)])
-        while s.shape[axis] > 1:
-            n = s.shape[axis]
+        if t.shape[axis] == 0:
+            t = t.new_zeros([1 if i == axis else n for i, n in enumerate(t.shape)])
+        while t.shape[axis] > 1:
+            n = t.shape[axis]
             half = (n + 1) // 2
-            low, high = s.narrow(axis, 0, half), s.narrow(axis, half, n - half)
-            s = low + high if n == 2 * half else _cat_last(low, high, axis)
-    return s.to(t.dtype).reshape(shape)
-
-
-def _cat_last(low, high, axis):
-    """low + high with one slice of low left over at the end."""
-    res = low.clone()
-    res.narrow(axis, 0, high.shape[axis]).add_(high)
-    return res
+            low, high = t.narrow(axis, 0, half), t.narrow(axis, half, n - half)
+            t = low.to(_torch_module.float64, copy=True)
+            t.narrow(axis, 0, n - half).add_(high)
+    return t.reshape(shape)
 
 
 def _observations(x, batch, torch, device):
@@ -396,8 +396,8 @@ def _observations(x, batch, torch, device):
     return t.contiguous(), _x_codes[t.dtype]
 
 
-def _value_dtype(z, torch):
-    return torch.float64 if z.dtype is torch.float64 else torch.float32
+def _value_dtype(dtype, torch):
+    return torch.float64 if dtype is torch.float64 else torch.float32
 
 
 def logpdf(x, logits):
@@ -408,7 +408,7 @@ def logpdf(x, logits):
         batch, k = t.shape[:-1], t.shape[-1]
         z, stride = _rows(t)
         xt, xcode = _observations(x, batch, torch, device)
-        out = torch.empty(batch, dtype=_value_dtype(z, torch), device=device)
+        out = torch.empty(batch, dtype=_value_dtype(z.dtype, torch), device=device)
         if z.shape[0]:
             _lib.check(L.m355_logits_logpdf(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, xt.data_ptr(), xcode,
                                             out.data_ptr(), _stream(torch, device)))
@@ -428,7 +428,7 @@ def sum_logpdf(x, logits, weights, grad, out=None):
         xt, xcode = _observations(x, batch, torch, device)
         keep = []
         w = _pack_operand(*_row_operand(1.0 if weights is None else weights, batch, torch, device, keep, "weights"))
-        total = torch.empty((), dtype=_value_dtype(z, torch), device=device)
+        total = torch.empty((), dtype=_value_dtype(z.dtype, torch), device=device)
         rows, code = z.shape[0], _codes[z.dtype]
         dz, o, ostride = None, None, 0
         if grad and out is None:

@@ -52,6 +52,7 @@ def adjust(logits, history=None, lengths=None, prompt_lengths=None, repetition=1
 def adjust_grad(g, logits, history=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
                 bias=None, temperature=1.0, mask=None):
     """(gradient with respect to the logits, with respect to the bias or None) of adjust(logits, ...) for the gradient g of
-    its result (g is converted to the logits' dtype); each has the shape and dtype of its argument.  Penalties, temperature and mask are data.  A bias that
-    several rows share gets the sum over them, added in a fixed order.  Not allowed: 0, whatever g holds there."""
+    its result (g is converted to the logits' dtype); each has the shape and dtype of its argument.  Penalties, temperature
+    and mask are data.  A bias that rows share, all of them or along some of their axes, gets the sum over them, added in
+    float64 in a fixed order.  Not allowed: 0, whatever g holds there."""
     return _adjust_grad(g, logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask)

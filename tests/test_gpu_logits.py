@@ -699,6 +699,31 @@ def test_bias_shared_by_some_axes(gpu):
             assert torch.equal(captured, cl.adjust_grad(g, z, bias=bias)[1])
 
 
+@pytest.mark.parametrize("bdt", DT)
+@pytest.mark.parametrize("dt", DT)
+def test_bias_shared_along_a_long_axis(gpu, dt, bdt):
+    """The sum over the rows that share a bias is rounded to the bias' type once, whatever that is and whichever axes it has."""
+    from distributions_amd import categorical_logits as cl
+
+    dtype, b_dtype, k = DT[dt], DT[bdt], 37
+    u, ut, tiny = steps(dtype)[0], *steps(b_dtype)[1:]
+    if dt != "f64":
+        u = 2.0**-24
+    for shape, bshape in (((2, 1500, k), (2, 1, k)), ((1500, 2, k), (2, k)), ((40, 3, 40, k), (1, 3, 1, k)), ((3000, k), (k,))):
+        g, z = make(shape, dtype, 1, gpu), make(shape, dtype, 2, gpu)
+        bias = make(bshape, b_dtype, 3, gpu)
+        t = (0.5 + torch.rand(shape[:-1], generator=torch.Generator().manual_seed(4))).to(gpu)
+        _, db = cl.adjust_grad(g, z, bias=bias, temperature=t)
+        assert db.dtype == b_dtype and db.shape == bshape
+        terms = g.cpu().double() / t.cpu().double()[..., None]
+        full = (1,) * (len(shape) - len(bshape)) + bshape
+        axes = [i for i, (m, n) in enumerate(zip(full, shape)) if m != n]
+        ref, size = terms.sum(axes).reshape(bshape), terms.abs().sum(axes).reshape(bshape)
+        # each term: 1 / T and its product, 2 u; float64 additions: 3000 * 2^-53; then the rounding to the bias' type, for 16
+        # bits by way of float32 (u), and from float32 where the kernel's output is that
+        within(db, ref, ut * ref.abs() + 2 * 2.0**-24 * ref.abs() * (bdt != "f64" or dt != "f64") + (2 * u + 3000 * 2.0**-53) * size + tiny)
+
+
 def test_two_streams_at_once(gpu):
     """Steps of two problems that are under way together on two streams give what each gives alone."""
     work, want = [], []
