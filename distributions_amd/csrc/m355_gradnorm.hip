@@ -126,7 +126,14 @@ M355_DEV void store_norm(void* norm, int dtype, double v) {
   else *static_cast<float*>(norm) = (float)v;
 }
 
-// Joins the partial sums: the sum of squares, the norm, and the factor of the clipping (1: nothing is clipped)
+// The factor of the clipping, 1 where nothing is clipped: up to max_norm, and where the norm is not finite as it goes out (the
+// sum of squares of float32 gradients may have a root that float32 does not hold).
+M355_DEV double clip_factor(double n, double max_norm, int norm_dtype) {
+  const bool finite = norm_dtype == M355_F64 ? n < kInf : (float)n < (float)kInf;
+  return n > max_norm && finite ? max_norm / n : 1.0;
+}
+
+// Joins the partial sums: the sum of squares, the norm, and the factor of the clipping
 __global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __restrict__ partials, int count,
                                                               double* __restrict__ sumsq, void* __restrict__ norm,
                                                               int norm_dtype, double max_norm, double* __restrict__ factor) {
@@ -143,7 +150,7 @@ __global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __re
     const double n = ::sqrt(s);
     if (sumsq) *sumsq = s;
     store_norm(norm, norm_dtype, n);
-    if (factor) *factor = n > max_norm && n < kInf ? max_norm / n : 1.0;
+    if (factor) *factor = clip_factor(n, max_norm, norm_dtype);
   }
 }
 
@@ -200,8 +207,7 @@ __global__ __launch_bounds__(kFinalThreads) void k_norm_small(const TensorList l
   }
   if (!scales) return;
   __syncthreads();
-  const double n = ::sqrt(shared_sum);
-  const double f = n > max_norm && n < kInf ? max_norm / n : 1.0;
+  const double f = clip_factor(::sqrt(shared_sum), max_norm, norm_dtype);
   for (int c = lo; c < hi; ++c) {
     const int t = tensor_of(l, c);
     if (f == 1.0 && l.in[t] == l.out[t]) continue;

@@ -16,7 +16,8 @@ def global_norm(grads):
 
 def clip_global_norm(grads, max_norm, out=None):
     """(norm, clipped gradients): every gradient times max_norm / norm where norm > max_norm, unchanged otherwise and where
-    the norm is not finite (nothing is scaled by 0 or NaN: the caller sees the norm).  max_norm is a number >= 0.  out: list
+    the norm that is returned is not finite (nothing is scaled by 0 or NaN: the caller sees the norm; a float32 norm is
+    infinite from 3.4e38 on).  max_norm is a number >= 0.  out: list
     of tensors that receive the result, in the gradients' order; out=grads clips in place.  Outputs that share memory with
     each other or with another gradient are refused."""
     return _clip(grads, max_norm, out)

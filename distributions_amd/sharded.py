@@ -62,7 +62,9 @@ def total_loglik(terms: Sequence[tuple], group=None):
 def clip_global_norm(grads, max_norm, out=None, group=None):
     """gradients.clip_global_norm over the gradients of all ranks: each rank passes its own shards (disjoint parts of the
     whole; a gradient that every rank holds would count once per rank), the sums of squares are added by one all-reduce of
-    8 bytes, and each rank scales its shards by the common factor.  Returns (norm over all ranks, clipped shards)."""
+    8 bytes, and each rank scales its shards by the common factor.  Returns (norm over all ranks, clipped shards); the norm
+    has the type that the rank's own list gives it, and past 3.4e38 a rank with a float64 among its gradients scales while one
+    without sees an infinite norm and does not."""
     from . import _gradnorm
 
     sumsq = _gradnorm.global_norm(grads, sumsq_only=True)

@@ -424,8 +424,8 @@ int m355_logits_sum_logpdf_grad(int64_t rows, int64_t k, int dtype, const void* 
  *   m355_global_norm       norm = sqrt(sum of all squares), the squares added in float64 in a fixed order; *sumsq (device,
  *                          or NULL) receives the sum, norm (device, norm_dtype F64 / F32, or NULL) its square root
  *   m355_clip_global_norm  out = norm > max_norm ? ptr * (max_norm / norm) : ptr, per tensor, one rounding; a norm that is
- *                          not finite scales nothing.  sumsq (device, one double) replaces the sum over `tensors` where it
- *                          is not NULL (a sum over the shards of several processes).  norm as above.
+ *                          not finite in norm_dtype scales nothing.  sumsq (device, one double) replaces the sum over
+ *                          `tensors` where it is not NULL (a sum over the shards of several processes).  norm as above.
  * out may be ptr itself; M355_ERR_INVALID if an output overlaps another tensor's memory.  workspace:
  * m355_global_norm_workspace_bytes(count) bytes, 8-byte aligned, scratch; calls that may run concurrently need one each.
  */

@@ -122,6 +122,31 @@ def test_large_small_and_not_finite_values(gpu):
     assert math.isfinite(float(n))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [8, 300000])  # one workgroup, and the general launches
+def test_norm_that_float32_does_not_hold(gpu, dtype, n):
+    """Finite gradients whose norm is returned as infinite are left as they are: what is returned and what is done agree."""
+    from distributions_amd import gradients as G
+    from distributions_amd import sharded
+
+    for value, finite in ((3e38, False), (1e38 / math.sqrt(n), True)):
+        grads = [torch.full((n,), value, dtype=dtype, device=gpu), torch.zeros(5, dtype=dtype, device=gpu)]
+        before = [g.clone() for g in grads]
+        for clip in (G.clip_global_norm, sharded.clip_global_norm):
+            norm, clipped = clip(grads, 1.0)
+            assert norm.dtype == torch.float32 and bool(norm.isfinite()) == finite
+            assert torch.equal(clipped[0], before[0]) != finite and torch.equal(norm, G.global_norm(grads))
+            if finite:
+                check(norm, clipped, grads, [b.cpu().double() for b in before], 1.0)
+            inplace = [g.clone() for g in grads]
+            clip(inplace, 1.0, out=inplace)
+            assert all(torch.equal(a, b) for a, b in zip(inplace, clipped))
+    # a float64 tensor in the list: the norm is float64 and finite, and everything is scaled
+    grads = [torch.full((n,), 3e38, dtype=dtype, device=gpu), torch.ones(3, dtype=torch.float64, device=gpu)]
+    norm, clipped = G.clip_global_norm(grads, 1.0)
+    check(norm, clipped, grads, [g.cpu().double() for g in grads], 1.0)
+
+
 def test_empty_lists_twice_listed_and_numpy(gpu):
     from distributions_amd import gradients as G
     from distributions_amd import normal
