@@ -81,8 +81,42 @@ template <class T> struct BiasPiece<T, void> {
   M355_DEV void add_to(typename T::comp (&)[kPer<T>]) const {}
 };
 
-// 1 / temperature of a row: one rounding more than a division per element, which would cost more than the rest of the body
-template <class C> M355_DEV C inverse_temperature(const AdjustArgs& a, long long row) { return (C)1 / (C)row_operand(a.temp, row); }
+// Quotients by a row's argument d (temperature, repetition) are products with its reciprocal: one rounding more than a
+// division per element, which would cost more than the rest of the body.  That needs a reciprocal that is a normal number:
+// |d| in [2^-126, 2^126] (float64: 2^-1022, 2^1022).
+template <class C> M355_DEV C reciprocal(const DevOperand& o, long long row) { return (C)1 / (C)row_operand(o, row); }
+template <class C> M355_DEV bool normal(C inv) {
+  constexpr C lo = (C)(sizeof(C) == 8 ? 0x1p-1022 : 0x1p-126);
+  return __builtin_fabs(inv) >= lo && __builtin_fabs(inv) <= 1 / lo;
+}
+M355_DEV float ldexp_c(float v, int e) { return __builtin_ldexpf(v, e); }
+M355_DEV double ldexp_c(double v, int e) { return __builtin_ldexp(v, e); }
+// Products with d and 1 / d for any d = m 2^e: the power of two first, by the exponent, and m such that this overflows only
+// where the result does.  For |d| in the range above the same values as the short way; 0, infinities and NaN as in s * d, s / d.
+template <class C> struct Factor {
+  C mul, inv;
+  int up = 0, down = 0;
+  M355_DEV explicit Factor(double d) : mul((C)d), inv((C)1 / (C)d) {
+    if (normal(inv)) return;
+    const double m = __builtin_amdgcn_frexp_mant(d);
+    const int e = __builtin_amdgcn_frexp_exp(d);
+    mul = (C)(2 * m), inv = (C)1 / (C)m;
+    up = e - 1, down = -e;
+  }
+  M355_DEV C times(C s) const { return ldexp_c(s, up) * mul; }
+  M355_DEV C over(C s) const { return ldexp_c(s, down) * inv; }
+};
+// s / argument of the row; inv: its reciprocal
+template <class C, int N> M355_DEV void divide(C (&s)[N], const DevOperand& o, long long row, C inv) {
+  if (__builtin_expect(normal(inv), true)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] *= inv;
+    return;
+  }
+  const Factor<C> f(row_operand(o, row));
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] = f.over(s[e]);
+}
 
 struct AdjustGrid {
   long long items;
@@ -151,11 +185,13 @@ M355_DEV void count_history(const AdjustArgs& a, long long row, unsigned base, u
 template <class C> struct Penalties {
   C rep, inv, pres, freq;
   M355_DEV C factor(C x) const { return x > 0 ? inv : rep; }
-  M355_DEV C operator()(C s, unsigned count) const {
-    const C p = s * factor(s);
-    s = count ? p : s;
+  M355_DEV C counted(C s, unsigned count) const {
     const C q = s - (freq * (C)(count >> 1) + pres);
     return count >> 1 ? q : s;
+  }
+  M355_DEV C operator()(C s, unsigned count) const {
+    const C p = s * factor(s);
+    return counted(count ? p : s, count);
   }
 };
 
@@ -174,7 +210,7 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
   constexpr int kCounts = HIST ? (THREADS * VPT + 1) * N : 4;  // one piece more for the tail
   __shared__ uint4 count_store[(kCounts * sizeof(cnt) + 15) / 16];
   cnt* counts = reinterpret_cast<cnt*>(count_store);
-  const int tid = threadIdx.x, nv = (int)(a.k / N), tail = (int)(a.k - (long long)nv * N);
+  const int tid = threadIdx.x, nv = (int)(a.k / N);
   for (long long item = blockIdx.x; item < grid.items; item += gridDim.x) {
     long long row;
     int chunk;
@@ -182,8 +218,7 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
     const int c0 = chunk * grid.per, c1 = c0 + grid.per < nv ? c0 + grid.per : nv;  // pieces of the chunk
     const long long base = (long long)c0 * N;
     const unsigned count_here = (unsigned)(c1 - c0);
-    const bool has_tail = chunk == grid.chunks - 1 && tid < tail;
-    const long long vt = (long long)nv * N + tid;
+    const unsigned width = chunk == grid.chunks - 1 ? (unsigned)(a.k - base) : count_here * N;  // categories of the chunk
     const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
     raw_t<T> raw[VPT];
     MaskPiece<T> mask[VPT];
@@ -197,7 +232,7 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
       bias[j].load(a, row, base, i * N);
     }
     // the row's arguments before the barriers: behind them their latency would stand alone
-    const comp inv_t = inverse_temperature<comp>(a, row);
+    const comp inv_t = reciprocal<comp>(a.temp, row);
     Penalties<comp> penalty = {1, 1, 0, 0};
     if constexpr (HIST) {
       penalty.rep = (comp)row_operand(a.rep, row);
@@ -206,18 +241,19 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
       penalty.freq = (comp)row_operand(a.freq, row);
       for (int i = tid; i < (int)(sizeof(count_store) / 16); i += THREADS) count_store[i] = uint4{0, 0, 0, 0};
       __syncthreads();
-      const long long left = a.k - base;
-      const unsigned width = chunk == grid.chunks - 1 ? (unsigned)left : (unsigned)((c1 - c0) * N);
       if (a.history_dtype == M355_I64) count_history<cnt, long long, THREADS>(a, row, (unsigned)base, width, reinterpret_cast<unsigned*>(counts));
       else count_history<cnt, int, THREADS>(a, row, (unsigned)base, width, reinterpret_cast<unsigned*>(counts));
       __syncthreads();
     }
     store* dst = static_cast<store*>(a.dst) + row * a.dst_ld;
     const store* x = static_cast<const store*>(a.x) + row * a.x_ld;
+    // behind the barriers: the arguments' loads are not waited for before the ids are under way
+    const bool fast = normal(inv_t) && normal(penalty.inv);
+    const unsigned whole = fast ? count_here : 0;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const unsigned i = j * THREADS + tid, rel = i * N;
-      if (i >= count_here) continue;
+      if (i >= whole) continue;
       comp s[N];
       unpack<T>(raw[j], s);
       cnt count[N];
@@ -246,10 +282,10 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
         if constexpr (!std::is_void<B>::value) {  // every row has its own bias: the gradient goes out as it is
 #pragma unroll
           for (int h = 0; h < N; h += kPer<B>) {
-            typename B::comp t[kPer<B>];
+            typename B::comp db[kPer<B>];
 #pragma unroll
-            for (int e = 0; e < kPer<B>; ++e) t[e] = (typename B::comp)s[h + e];
-            store_raw_nt<B>(static_cast<typename B::store*>(a.dbias) + row * a.k + base + (rel + h), pack<B>(t));
+            for (int e = 0; e < kPer<B>; ++e) db[e] = (typename B::comp)s[h + e];
+            store_raw_nt<B>(static_cast<typename B::store*>(a.dbias) + row * a.k + base + (rel + h), pack<B>(db));
           }
         }
         if (a.dst) {
@@ -262,23 +298,35 @@ __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a
         }
       }
     }
-    if (has_tail) {
-      const unsigned count = HIST ? counts[vt - base] : 0;
-      comp s = (comp)src[vt];
-      const bool ok = allowed(a, row, vt);
-      if constexpr (!BWD) {
-        s = penalty(s, count);
-        if constexpr (!std::is_void<B>::value) s += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + vt];
-        dst[vt] = (store)(ok ? s * inv_t : (comp)-kInf);
-      } else {
-        s = ok ? s * inv_t : (comp)0;
-        if constexpr (!std::is_void<B>::value)
-          static_cast<typename B::store*>(a.dbias)[row * a.k + vt] = (typename B::store)s;
-        if (a.dst) {
-          if (count) s *= penalty.factor((comp)x[vt]);
-          dst[vt] = (store)s;
+    auto single = [&](unsigned rel, auto exact) {
+      const unsigned count = HIST ? counts[rel] : 0;
+      const long long v = base + rel;
+      const comp t = (comp)src[v];
+      const bool ok = allowed(a, row, v);
+      auto over_t = [&](comp s) { return exact ? Factor<comp>(row_operand(a.temp, row)).over(s) : s * inv_t; };
+      auto repeated = [&](comp s, comp z) {
+        if constexpr (exact) {
+          const Factor<comp> r(row_operand(a.rep, row));
+          return z > 0 ? r.over(s) : r.times(s);
         }
+        return s * penalty.factor(z);
+      };
+      if constexpr (!BWD) {
+        comp s = HIST && count ? repeated(t, t) : t;
+        if constexpr (HIST) s = penalty.counted(s, count);
+        if constexpr (!std::is_void<B>::value) s += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + v];
+        dst[v] = (store)(ok ? over_t(s) : (comp)-kInf);
+      } else {
+        const comp s = ok ? over_t(t) : (comp)0;
+        if constexpr (!std::is_void<B>::value) static_cast<typename B::store*>(a.dbias)[row * a.k + v] = (typename B::store)s;
+        if (a.dst) dst[v] = (store)(HIST && count ? repeated(s, (comp)x[v]) : s);
       }
+    };
+    if (__builtin_expect(fast, true)) {
+      const unsigned rel = count_here * N + tid;
+      if (rel < width) single(rel, std::false_type());
+    } else {
+      for (unsigned rel = tid; rel < width; rel += THREADS) single(rel, std::true_type());
     }
     if constexpr (HIST) __syncthreads();  // the next item clears the counts
   }
@@ -295,7 +343,7 @@ template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_l
     const long long row = all <= 0xffffffffll ? (unsigned)p / (unsigned)pieces : p / pieces;
     const int i = (int)(p - row * pieces);
     const store* src = static_cast<const store*>(a.src) + row * a.src_ld;
-    const comp inv_t = inverse_temperature<comp>(a, row);
+    const comp inv_t = reciprocal<comp>(a.temp, row);
     comp s[N], b[N];
     bool ok[N];
     if (i < nv) {
@@ -318,10 +366,11 @@ template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_l
           s[e] += (comp) static_cast<const typename B::store*>(a.bias)[row * a.bias_ld + v];
       }
     }
+    divide(s, a.temp, row, inv_t);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const int v = i * N + e;
-      if (v < k) b[e] = ok[e] ? s[e] * inv_t : BWD ? (comp)0 : (comp)-kInf;
+      if (v < k) b[e] = ok[e] ? s[e] : BWD ? (comp)0 : (comp)-kInf;
     }
     if constexpr (BWD && !std::is_void<B>::value) {
 #pragma unroll
@@ -363,6 +412,7 @@ __global__ __launch_bounds__(kSumThreads) void k_logits_adjust_cols(const Adjust
   double acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.0;
+  bool all_normal = true;
   if (i < nv) {
     const long long v = (long long)i * N;
     for (long long first = lo + group; first < hi; first += G * kSumRows) {
@@ -375,7 +425,8 @@ __global__ __launch_bounds__(kSumThreads) void k_logits_adjust_cols(const Adjust
         if (row >= hi) continue;
         raw[r] = __builtin_nontemporal_load(reinterpret_cast<const raw_t<T>*>(static_cast<const store*>(a.src) + row * a.src_ld + v));
         mask[r].load(a, row, 0, (unsigned)v);
-        inv_t[r] = inverse_temperature<comp>(a, row);
+        inv_t[r] = reciprocal<comp>(a.temp, row);
+        all_normal = all_normal && normal(inv_t[r]);
       }
 #pragma unroll
       for (int r = 0; r < kSumRows; ++r) {
@@ -391,11 +442,32 @@ __global__ __launch_bounds__(kSumThreads) void k_logits_adjust_cols(const Adjust
         if constexpr (WRITE) store_raw_nt<T>(static_cast<store*>(a.dst) + row * a.dst_ld + v, pack<T>(s));
       }
     }
-  } else if (i - nv < tail) {
+  }
+  // Temperatures without a normal reciprocal: the thread's rows once more.  (A branch in the loop above keeps the rows' loads
+  // from overlapping: 4096 x 32768 bf16 132 against 126 us; a look at the temperatures before it costs 1.2 us.)
+  if (__builtin_expect(i < nv && !all_normal, false)) {
+    const long long v = (long long)i * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.0;
+    for (long long row = lo + group; row < hi; row += G) {
+      const Factor<comp> t(row_operand(a.temp, row));
+      MaskPiece<T> mask;
+      mask.load(a, row, 0, (unsigned)v);
+      comp s[N];
+      unpack<T>(load_raw<T>(static_cast<const store*>(a.src) + row * a.src_ld + v), s);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        s[e] = mask(a, e) ? t.over(s[e]) : (comp)0;
+        acc[e] += (double)s[e];
+      }
+      if constexpr (WRITE) store_raw_nt<T>(static_cast<store*>(a.dst) + row * a.dst_ld + v, pack<T>(s));
+    }
+  }
+  if (i >= nv && i - nv < tail) {
     const long long v = (long long)nv * N + (i - nv);
     for (long long row = lo + group; row < hi; row += G) {
-      const comp s = allowed(a, row, v) ? (comp) static_cast<const store*>(a.src)[row * a.src_ld + v] * inverse_temperature<comp>(a, row)
-                                        : (comp)0;
+      const comp g = (comp) static_cast<const store*>(a.src)[row * a.src_ld + v];
+      const comp s = allowed(a, row, v) ? Factor<comp>(row_operand(a.temp, row)).over(g) : (comp)0;
       acc[0] += (double)s;
       if constexpr (WRITE) static_cast<store*>(a.dst)[row * a.dst_ld + v] = (store)s;
     }

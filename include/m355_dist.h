@@ -391,7 +391,8 @@ int m355_logits_adjust(int64_t rows, int64_t k, int dtype, const void* logits, i
  *     dlogits = allowed ? g / temperature * (c_all > 0 ? (z > 0 ? 1 / repetition : repetition) : 1) : 0
  *     dbias   = allowed ? g / temperature : 0, per element (bias_stride != 0: rows x k contiguous values of bias_dtype)
  *               or summed over the rows in a fixed order, in float64 (bias_stride == 0: k values, k <= 2^28)
- * dlogits (rows x k contiguous) or dbias may be NULL: not wanted.  logits is read only with a history.  workspace:
+ * dlogits (rows x k contiguous) or dbias may be NULL: not wanted.  logits is read only with a history.  An output that
+ * overlaps an input is undefined.  workspace:
  * m355_logits_adjust_grad_workspace_bytes bytes, 8-byte aligned, needed with dbias and bias_stride 0; scratch.  With no rows
  * that is none, and the dbias that all rows share becomes 0.
  */

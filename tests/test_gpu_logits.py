@@ -233,6 +233,112 @@ def test_adjust_infinities_nan_and_lowest_values(gpu):
         within(cl.adjust(torch.ones(1, 9, dtype=dtype, device=gpu), bias=lowest), torch.full((1, 9), low, dtype=torch.float64), abs(low) * 2.0**-7)
 
 
+def ends_of_the_range(dt):
+    """Positive arguments whose reciprocal, or which themselves, are no normal numbers of the arithmetic, and some that are."""
+    if dt == "f64":
+        return [1.0, 5e-324, 1e-309, 2.0**-1022 * 0.75, 2.0**-1022, 2.0**1022, 2.0**1022 * 1.5, 1.7e308, 0.7]
+    return [1.0, 1e-300, 1e-60, 1.4e-45, 1e-39, 2.0**-126 * 0.75, 2.0**-126, 2.0**126, 2.0**126 * 1.5, 3e38, 1e39, 1e60, 0.7]
+
+
+def values_for(args, rows, k, dtype, seed):
+    """Values of all sizes, zeros and infinities, whose quotients by and products with `args` (one per row) stay off the border
+    where the type, or float32 before it, overflows."""
+    gen = torch.Generator().manual_seed(seed)
+    top, low = math.log2(torch.finfo(dtype).max), math.log2(torch.finfo(dtype).tiny)
+    x = torch.exp2(low + (top - 1 - low) * torch.rand(rows, k, generator=gen, dtype=torch.float64))
+    x *= torch.sign(torch.randn(rows, k, generator=gen, dtype=torch.float64))
+    x = x.to(dtype).double()
+    small = torch.rand(rows, k, generator=gen) < 0.5
+    x = torch.where(small, torch.randn(rows, k, generator=gen).to(dtype).double(), x)
+    for q in (x / args, x * args):
+        for edge in (top, 128 if dtype != torch.float64 else top):
+            x = torch.where((torch.log2(q.abs()) - edge).abs() < 0.1, 0.0, x)
+    x[:, 0], x[:, 1 % k] = 0.0, -0.0
+    if k > 4:
+        x[:, 2], x[:, 3] = INF, -INF
+    return x.to(dtype)
+
+
+def in_range(ref, dtype):
+    """What rounds past the type's largest value (from half a step above it) is infinite."""
+    return torch.where(ref.to(dtype).isinf(), torch.sign(ref) * INF, ref)
+
+
+@pytest.mark.parametrize("k", [3, 101, 5003])
+@pytest.mark.parametrize("dt", DT)
+def test_arguments_at_the_ends_of_the_range(gpu, dt, k):
+    """Temperatures and repetition penalties without a normal reciprocal: 0 / T is 0 and x / T what it is, whatever T > 0."""
+    from distributions_amd import categorical_logits as cl
+
+    dtype = DT[dt]
+    u, ut, tiny = steps(dtype)
+    least = 2.0**-1074 if dt == "f64" else 2.0**-149
+    ends = torch.tensor(ends_of_the_range(dt), dtype=torch.float64)
+    args = ends.repeat(6)[:, None]
+    rows = len(args)
+    z, g = values_for(args, rows, k, dtype, 1), values_for(args, rows, k, dtype, 2)
+    h = torch.arange(0, k, 2).expand(rows, -1).contiguous()
+    seen = torch.zeros(rows, k, dtype=torch.bool)
+    seen[:, ::2] = True
+    zd, gd = z.double(), g.double()
+    # the argument, its reciprocal, the product; a result or, before the reciprocal's factor of at most 2, a power of two taken
+    # from the value may be subnormal: half a step times 2 and another half
+    bound = lambda ref: (ut + 3 * u) * torch.nan_to_num(ref, posinf=0.0, neginf=0.0).abs() + tiny + 1.5 * least  # noqa: E731
+    z, g, t = z.to(gpu), g.to(gpu), args[:, 0].to(gpu)
+    by_t = in_range(zd / args, dtype)
+    for history in (None, h.to(gpu)):
+        within(cl.adjust(z, history=history, temperature=t), by_t, bound(by_t))
+        ref = in_range(gd / args, dtype)
+        dz, db = cl.adjust_grad(g, z, history=history, temperature=t, bias=torch.zeros_like(z))
+        within(dz, ref, bound(ref))
+        within(db, ref, bound(ref))
+    by_rep = in_range(torch.where(seen, torch.where(zd > 0, zd / args, zd * args), zd), dtype)
+    within(cl.adjust(z, history=h.to(gpu), repetition=t), by_rep, bound(by_rep))
+    by_rep = in_range(torch.where(seen, torch.where(zd > 0, gd / args, gd * args), gd), dtype)
+    within(cl.adjust_grad(g, z, history=h.to(gpu), repetition=t)[0], by_rep, bound(by_rep))
+    # one argument for all rows, as a Python number (and as float32 where that holds it)
+    for v in ends.tolist():
+        ref = in_range(zd / v, dtype)
+        ok = ((torch.log2(ref.abs()) - math.log2(torch.finfo(dtype).max)).abs() > 0.1) & ((torch.log2(ref.abs()) - 128).abs() > 0.1) | (ref == INF)
+        ref = torch.where(ok | ~ref.isfinite(), ref, 0.0)
+        zz = torch.where(ok | ~ref.isfinite(), z.cpu(), torch.zeros_like(z.cpu())).to(gpu)
+        within(cl.adjust(zz, temperature=v), ref, bound(ref))
+
+
+@pytest.mark.parametrize("k", [3, 101, 5003])
+@pytest.mark.parametrize("dt", DT)
+def test_shared_bias_with_temperatures_at_the_ends_of_the_range(gpu, dt, k):
+    """The column sums of the same: few rows of such temperatures among others, with and without a history."""
+    from distributions_amd import categorical_logits as cl
+
+    dtype = DT[dt]
+    u, ut, tiny = steps(dtype)
+    least = 2.0**-1074 if dt == "f64" else 2.0**-149
+    ends = torch.tensor(ends_of_the_range(dt), dtype=torch.float64)
+    rows = 150
+    args = torch.full((rows, 1), 0.7, dtype=torch.float64)
+    args[7 : 7 + 11 * len(ends) : 11, 0] = ends
+    g = values_for(args, rows, k, dtype, 3)
+    g[:, 2:] = g[:, 2:].abs()  # infinities of one sign
+    g[:, 2:] = torch.where((g.double() / args).abs() < 1e30, g, torch.ones_like(g))[:, 2:] if dt != "f64" else g[:, 2:]
+    if dt == "f64":
+        g = torch.where((g.abs() / args < 1e300) | (g == 0), g, torch.zeros_like(g))
+    small = args[:, 0] < 1e-20
+    g[small] = 0.0  # 0 / T is 0, and not NaN
+    ref = g.double() / args
+    assert bool(ref.isfinite().all())
+    size = ref.abs().sum(0)
+    zero = torch.zeros(rows, k, dtype=dtype, device=gpu)
+    wide = torch.float64 if dt == "f64" else torch.float32
+    for history in (None, torch.zeros(rows, 3, dtype=torch.int64, device=gpu)):
+        dz, db = cl.adjust_grad(g.to(gpu), zero, history=history, temperature=args[:, 0].to(gpu), bias=torch.zeros(k, dtype=wide, device=gpu))
+        rd = in_range(ref, dtype)
+        within(dz, rd, (ut + 3 * u) * torch.nan_to_num(rd, posinf=0.0, neginf=0.0).abs() + tiny + 1.5 * least)
+        # terms as above, float64 additions, float32 result
+        total = in_range(ref.sum(0), wide)
+        within(db, total, 4 * u * size + rows * 2.0**-53 * size + rows * 2 * least)
+
+
 def test_adjust_long_and_degenerate_histories(gpu):
     from distributions_amd import categorical_logits as cl
 
