@@ -607,6 +607,149 @@ def test_many_short_rows(gpu):
         within(db, rb, 3 * u * rb.abs() + 2.0**-149)
 
 
+# the borders between launch variants of the density and its gradient: row lengths in pieces of 16 bytes are 2^8 ... 2^14 for
+# one type or another, one piece more, and a tail behind it
+BORDERS = [512, 520, 1024, 1037, 2048, 2057, 4096, 4107, 8192 + 8, 10007, 16384, 16395, 32768, 32779, 65536, 65541, 131080]
+
+
+@pytest.mark.parametrize("k", BORDERS)
+@pytest.mark.parametrize("dt", DT)
+def test_density_at_the_borders_of_its_variants(gpu, dt, k):
+    from distributions_amd import categorical_logits as cl
+
+    z = make((4, k), DT[dt], k, gpu)
+    x = torch.tensor([k - 1, 0, k // 2, k - 9])
+    w = torch.tensor([1.0, -0.5, 2.0, 0.25], dtype=torch.float64 if dt == "f64" else torch.float32)
+    lp, b_lp, total, b_total, grad, b_g = plain_logpdf(x, z, w)
+    within(cl.logpdf(x.to(gpu), z), lp, b_lp)
+    t, (_, g) = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    within(t, total, b_total)
+    within(g, grad, b_g)
+    t2, (_, g2) = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu), out=z)
+    assert g2 is z and torch.equal(g2, g) and torch.equal(t2, t)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_many_long_rows(gpu, dt):
+    """From 1024 rows on, longer than the value's kernel of 256 threads holds at once."""
+    from distributions_amd import categorical_logits as cl
+
+    rows, k = 1030, 9001
+    z = make((rows, k), DT[dt], 3, gpu)
+    x = torch.arange(rows) * 8 % k
+    lp, b_lp, *_ = plain_logpdf(x, z)
+    within(cl.logpdf(x.to(gpu), z), lp, b_lp)
+
+
+@pytest.mark.parametrize("rows, k", [(8192, 3), (8193, 3), (20000, 40), (12289, 600)])
+@pytest.mark.parametrize("dt", DT)
+def test_total_over_many_rows(gpu, dt, rows, k):
+    """From 8193 rows on several workgroups add the rows, and a last one what they have added."""
+    from distributions_amd import categorical_logits as cl
+
+    z = make((rows, k), DT[dt], 1, gpu)
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randint(0, k, (rows,), generator=gen)
+    w = torch.randn(rows, generator=gen, dtype=torch.float64 if dt == "f64" else torch.float32)
+    w[::7] = 0
+    x[::7] = -1  # padding
+    _, _, total, b_total, grad, b_g = plain_logpdf(x, z, w)
+    within(cl.sum_logpdf(x.to(gpu), z, w.to(gpu)), total, b_total)
+    t, (_, g) = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    within(t, total, b_total)
+    within(g, grad, b_g)
+    again, _ = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    assert torch.equal(again, t)
+
+
+@pytest.mark.parametrize("history", [0, 3])
+@pytest.mark.parametrize("rows, k", [(5003, 1), (5003, 10), (5003, 100), (700, 257), (5003, 2051)])
+@pytest.mark.parametrize("dt", DT)
+def test_shared_bias_gradient_over_many_rows(gpu, dt, rows, k, history):
+    """Column sums of few columns over several blocks of rows."""
+    from distributions_amd import categorical_logits as cl
+
+    dtype, wide = DT[dt], torch.float64 if dt == "f64" else torch.float32
+    u, ut, tiny = steps(dtype)
+    z, g = make((rows, k), dtype, 1, gpu), make((rows, k), dtype, 2, gpu)
+    a = adjust_args(rows, k, 5, gpu, history, "bool" if k != 100 else "bits", "shared", wide)
+    dz, db = cl.adjust_grad(g, z, **a)
+    rz, rb = plain_adjust_grad(g, z, **a)
+    within(dz, rz, ut * rz.abs() + 6 * u * rz.abs() + tiny)
+    # terms: T, 1 / T, the product; float64 additions, one after the other at worst; the result's own rounding
+    within(db, rb.sum(0), (4 * u + rows * 2.0**-53) * rb.abs().sum(0) + 2.0**-149)
+    assert torch.equal(db, cl.adjust_grad(g, z, **a)[1])
+
+
+def repeated(base, rows):
+    return base.repeat((rows // len(base) + 1,) + (1,) * (base.dim() - 1))[:rows]
+
+
+def same_as_repeated(got, base):
+    """Whether `got` is `base` again and again, compared without another copy of it."""
+    n = len(got) // len(base) * len(base)
+    return bool((got[:n].view(-1, *base.shape) == base).all()) and torch.equal(got[n:], base[: len(got) - n])
+
+
+@pytest.mark.parametrize("rows, k", [(2**21 + 3001, 520), (2**23 + 777, 129), (2**27 + 777, 2)])
+def test_density_of_more_rows_than_workgroups(gpu, rows, k):
+    """Workgroups that walk on to further rows (there are 2^21 at most): every row as in a launch that has one for each."""
+    from distributions_amd import categorical_logits as cl
+
+    n = 1021
+    z = make((n, k), torch.bfloat16, 1, gpu)
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randint(0, k, (n,), generator=gen, dtype=torch.int32)
+    w = torch.randn(n, generator=gen)
+    w[::7], x[3::11] = 0.0, -1
+    lp, b_lp, _, _, grad, b_g = plain_logpdf(x, z, w)
+    lp0 = cl.logpdf(x.to(gpu), z)
+    within(lp0, lp, b_lp)
+    _, (_, g0) = cl.sum_logpdf_grad(x.to(gpu), z, w.to(gpu))
+    within(g0, grad, b_g)
+    big_z, big_x = repeated(z, rows), repeated(x.to(gpu), rows)
+    w[3::11] = 0.0  # a finite total
+    big_w = repeated(w.to(gpu), rows)
+    assert same_as_repeated(cl.logpdf(big_x, big_z), lp0)
+    total, (_, g) = cl.sum_logpdf_grad(big_x, big_z, big_w)
+    assert same_as_repeated(g, torch.where(w.to(gpu)[:, None] == 0, torch.zeros_like(g0), g0))
+    times = torch.full((n,), rows // n, dtype=torch.float64)
+    times[: rows % n] += 1
+    keep = w != 0
+    terms, off = (times * w.double() * lp)[keep], (times * w.double().abs() * b_lp)[keep]
+    # the rows' own bounds; float64 additions; the total's rounding
+    within(total, terms.sum(), float(off.sum() + (2 * 2.0**-24 + rows * 2.0**-53) * terms.abs().sum()))
+
+
+def test_adjust_of_more_rows_than_workgroups(gpu):
+    """The same for the adjustment: with a history (the counters in LDS are cleared between the rows), without one, and with
+    more pieces than 32 bits count."""
+    from distributions_amd import categorical_logits as cl
+
+    n, k, rows = 1021, 11, 2**21 + 3001
+    z = make((n, k), torch.bfloat16, 1, gpu)
+    a = adjust_args(n, k, 5, gpu, 6, "bool", "rows")
+    ref, bound = plain_adjust(z, **a)
+    small = cl.adjust(z, **a)
+    within(small, ref, bound)
+    dz0, db0 = cl.adjust_grad(z, z, **a)
+    big = {name: repeated(v, rows) for name, v in a.items()}
+    big_z = repeated(z, rows)
+    assert same_as_repeated(cl.adjust(big_z, **big), small)
+    dz, db = cl.adjust_grad(big_z, big_z, **big)
+    assert same_as_repeated(dz, dz0) and same_as_repeated(db, db0)
+    del dz, db, big, big_z
+    for rows, k in ((2**28 + 777, 3), (2**32 + 777, 1)):
+        z = make((n, k), torch.bfloat16, 1, gpu)
+        bias = make((k,), torch.bfloat16, 2, gpu)
+        small = cl.adjust(z, bias=bias, temperature=0.7)
+        ref, bound = plain_adjust(z, bias=bias, temperature=0.7)
+        within(small, ref, bound)
+        big = repeated(z, rows)
+        assert same_as_repeated(cl.adjust(big, bias=bias, temperature=0.7, out=big), small)
+        del big
+
+
 @pytest.mark.parametrize("k", [20, 3000])
 def test_weights_below_the_arithmetic(gpu, k):
     """A float64 weight that float32 rounds to 0 is no padding: its row counts in the total."""
