@@ -71,27 +71,6 @@ template <class T> M355_DEV raw_t<T> pack(const typename T::comp (&v)[kPer<T>]) 
   return r;
 }
 
-// Elements [v, v + kPer) of a row of k; those behind its end read as `fill`.  The common case is one 16-byte load; the
-// one vector that crosses the end loads its elements singly.
-template <class T>
-M355_DEV raw_t<T> load_row(const typename T::store* row, long long v, long long k, typename T::comp fill) {
-  if (v + kPer<T> <= k) return load_raw<T>(row + v);
-  typename T::comp t[kPer<T>];
-#pragma unroll
-  for (int e = 0; e < kPer<T>; ++e) t[e] = v + e < k ? (typename T::comp)row[v + e] : fill;
-  return pack<T>(t);  // every value came from (or fits) the storage type: nothing is rounded
-}
-template <class T>
-M355_DEV void store_row(typename T::store* row, long long v, long long k, const typename T::comp (&t)[kPer<T>]) {
-  if (v + kPer<T> <= k) {
-    *reinterpret_cast<raw_t<T>*>(row + v) = pack<T>(t);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < kPer<T>; ++e)
-    if (v + e < k) row[v + e] = (typename T::store)t[e];
-}
-
 // A per-row argument: scalar, or float64 / float32 array indexed by the row (mod == 0) or by (row / div) % mod
 M355_DEV double row_operand(const DevOperand& o, long long row) {
   if (!o.ptr) return o.scalar;
