@@ -160,6 +160,8 @@ def clip_global_norm(grads, max_norm, out=None, sumsq=None):
         for o, r in zip(given, outs):
             if o is not r:
                 o.detach().copy_(r)
+        if out is not None:
+            torch.autograd.graph.increment_version(given)  # autograd sees a write to what it may have saved
     res = list(given) if len(given) == len(ls.grads) else [None] * len(ls.grads)
     for i, o in zip(ls.places, given):
         res[i] = o if out is not None or isinstance(ls.grads[i], torch.Tensor) else o.cpu().numpy()

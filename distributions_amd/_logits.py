@@ -309,6 +309,8 @@ def adjust(logits, history, lengths, prompt_lengths, repetition, presence, frequ
         if z.shape[0]:
             _lib.check(L.m355_logits_adjust(z.shape[0], k, _codes[z.dtype], z.data_ptr(), stride, d, o.data_ptr(), ostride,
                                             _stream(torch, device)))
+        if out is not None:
+            torch.autograd.graph.increment_version(out)  # autograd sees a write to what it may have saved
         del keep
     return res if out is not None or _any_tensor(torch, *args) else res.cpu().numpy()
 
@@ -442,6 +444,8 @@ def sum_logpdf(x, logits, weights, grad, out=None):
         _lib.check(L.m355_logits_sum_logpdf_grad(rows, k, code, z.data_ptr(), stride, xt.data_ptr(), xcode, w, total.data_ptr(),
                                                  o.data_ptr() if grad and rows else None, ostride, ws.data_ptr(), need,
                                                  _stream(torch, device)))
+        if grad and out is not None:
+            torch.autograd.graph.increment_version(out)
         del keep
     if out is not None or _any_tensor(torch, logits, *args):
         return total, dz

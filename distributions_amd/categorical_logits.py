@@ -3,7 +3,8 @@ categorical.py takes one probability vector for all observations; there is no lo
 
 Logits have shape (..., k) in float64, float32, float16 or bfloat16, any strides; arithmetic and values (log-density, total)
 are float64 for float64 logits and float32 otherwise.  Inputs are torch CUDA tensors (torch results, nothing synchronises)
-or NumPy arrays (NumPy results).  csrc/m355_logits.hip."""
+or NumPy arrays (NumPy results).  Gradients are calls of their own here: nothing is recorded for autograd, which sees a write to
+`out` and no more.  csrc/m355_logits.hip."""
 
 from ._logits import adjust as _adjust
 from ._logits import adjust_grad as _adjust_grad

@@ -469,6 +469,30 @@ def test_out_in_place(gpu):
         assert g2 is y and torch.equal(y, grad) and torch.equal(t2, total)
 
 
+def test_outputs_count_as_writes(gpu):
+    """What autograd has saved and an output overwrites is an error in the backward pass, as with any operation in place."""
+    from distributions_amd import categorical_logits as cl
+    from distributions_amd import gradients
+
+    x = torch.tensor([1, 2, 3], device=gpu)
+    for write in (lambda y: cl.adjust(y, temperature=2.0, out=y), lambda y: cl.sum_logpdf_grad(x, y, out=y),
+                  lambda y: gradients.clip_global_norm([y], 0.1, out=[y]), lambda y: cl.adjust(y[1:], temperature=2.0, out=y[1:]),
+                  lambda y: gradients.clip_global_norm([y[:, 1:]], 0.1, out=[y[:, 1:]])):
+        leaf = torch.randn(3, 50, device=gpu, requires_grad=True)
+        y = leaf.exp()  # saves its result
+        before = y._version
+        write(y.detach())
+        assert y._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    z = torch.randn(3, 50, device=gpu)  # and nothing else does
+    cl.adjust(z, temperature=2.0), cl.sum_logpdf_grad(x, z), gradients.clip_global_norm([z], 0.1)
+    assert z._version == 0
+    with torch.inference_mode():
+        z = torch.randn(3, 50, device=gpu)
+        cl.adjust(z, temperature=2.0, out=z), gradients.clip_global_norm([z], 0.1, out=[z])
+
+
 # ------------------------------------------------------------------------------------------------- log-density
 @pytest.mark.parametrize("rows, k", SIZES + [(2, 50021), (1, 131072), (1, 262147), (300, 515), (700, 64), (5, 32), (9, 129), (4, 512), (3, 513)])
 @pytest.mark.parametrize("dt", DT)
