@@ -147,6 +147,22 @@ def test_norm_that_float32_does_not_hold(gpu, dtype, n):
     check(norm, clipped, grads, [g.cpu().double() for g in grads], 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tensor_of_more_than_2_to_the_31_elements(gpu, dtype):
+    """Offsets past 32 bits, of elements and of bytes, and the tensors behind such a one."""
+    from distributions_amd import gradients as G
+
+    big = torch.zeros(2**31 + 4099, dtype=dtype, device=gpu)
+    at = torch.tensor([0, 2**30 + 1, 2**31 - 1, 2**31 + 7, 2**31 + 4098], device=gpu)
+    big[at] = torch.tensor([2.0, 4.0, 2.0, 4.0, 2.0], dtype=dtype, device=gpu)  # squares: 44
+    grads = [torch.tensor([1.0], dtype=dtype, device=gpu), big, torch.tensor([2.0, 0.0], dtype=dtype, device=gpu)]
+    assert float(G.global_norm(grads)) == 7.0
+    norm, clipped = G.clip_global_norm(grads, 3.5, out=grads)
+    assert float(norm) == 7.0 and clipped[1] is big
+    assert big[at].tolist() == [1.0, 2.0, 1.0, 2.0, 1.0] and int(torch.count_nonzero(big)) == 5
+    assert grads[0].tolist() == [0.5] and grads[2].tolist() == [1.0, 0.0]
+
+
 def test_empty_lists_twice_listed_and_numpy(gpu):
     from distributions_amd import gradients as G
     from distributions_amd import normal
