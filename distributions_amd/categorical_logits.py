@@ -34,7 +34,7 @@ def sum_logpdf_grad(x, logits, weights=None, out=None):
 
 def adjust(logits, history=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
            temperature=1.0, mask=None, out=None):
-    """Logits as they are drawn from or scored: with c_all and c_gen the number of times category v stands in
+    """Logits as they are scored (by logpdf) or drawn from: with c_all and c_gen the number of times category v stands in
     history[..., :lengths] and history[..., prompt_lengths:lengths],
 
         s = logits;  where c_all > 0:  s = s / repetition if s > 0 else s * repetition
@@ -42,10 +42,9 @@ def adjust(logits, history=None, lengths=None, prompt_lengths=None, repetition=1
 
     history: integer ids (..., n), those outside [0, k) are skipped (padding); lengths, prompt_lengths: integers per row
     (default n and 0; clamped to [0, n]).  repetition, presence, frequency, temperature: numbers or arrays per row.  bias:
-    (k,) or (..., k), of the logits' dtype or float32 (other
-    types are converted).  mask: truth values (k,) or (..., k), or int32 words
-    (..., ceil(k / 32)) in which category v is bit v % 32 of word v // 32; true / 1 = allowed.  A row that allows nothing is
-    all -inf.  out: where the result goes; it may be the logits themselves.  Arrays with leading axes broadcast to
+    (k,) or (..., k), of the logits' dtype or float32 (other types are converted).  mask: truth values (k,) or (..., k), or
+    int32 words (..., ceil(k / 32)) in which category v is bit v % 32 of word v // 32; true / 1 = allowed.  A row that allows
+    nothing is all -inf.  out: where the result goes; it may be the logits themselves.  Arrays with leading axes broadcast to
     logits.shape[:-1]."""
     return _adjust(logits, history, lengths, prompt_lengths, repetition, presence, frequency, bias, temperature, mask, out)
 

@@ -100,7 +100,7 @@ template <class T> M355_DEV double sum_run(const TensorList& l, int lo, int hi, 
   return acc[0] + acc[1];
 }
 
-// The chunks of a launch in equal runs, one a workgroup.  Bound by HBM: 5.6e8 bytes of bf16 in 97 us, 5.7 TB/s.
+// The chunks of a launch in equal runs, one a workgroup.  Bound by HBM: 5.6e8 bytes of bf16 in 96-99 us, 5.7-5.9 TB/s.
 template <class T> __global__ __launch_bounds__(kListThreads) void k_norm_partials(const TensorList l, double* __restrict__ partials) {
   const int lo = (int)((long long)l.chunks * blockIdx.x / gridDim.x), hi = (int)((long long)l.chunks * (blockIdx.x + 1) / gridDim.x);
   const double s = block_reduce_sum(sum_run<T>(l, lo, hi, threadIdx.x));
@@ -177,7 +177,7 @@ template <class T> M355_DEV void scale_chunk(const TensorList& l, int t, int c, 
 }
 
 // One workgroup per chunk.  The list comes with its last tensors first: they are what the Infinity Cache still holds of the
-// pass that formed the norm.  5.55e8 bytes of bf16 read and written in 170-177 us, 6.3-6.5 TB/s, as a copy.
+// pass that formed the norm.  5.64e8 bytes of bf16 read and written in 170-190 us, 5.9-6.7 TB/s, as a copy.
 template <class T> __global__ __launch_bounds__(kListThreads) void k_norm_scale(const TensorList l, const double* __restrict__ factor) {
   const double f = *factor;
   for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {

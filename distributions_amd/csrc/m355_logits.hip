@@ -198,8 +198,10 @@ template <class C> struct Penalties {
 // One workgroup per (row, chunk): everything the chunk needs from memory is fetched first, then, with a history (CNT: the
 // type of its counters, or void), the ids that fall into the chunk are counted in LDS, then the pieces are worked off.  The
 // k % kPer last categories of a row belong to the first threads of its last chunk.  Without a history bound by HBM (1024 x
-// 65537 float32: 94 us, 5.7 TB/s, rows at odd addresses); with one by the chain ids -> counters -> barrier -> stores: 256 x
-// 100003 float32 with 4001 ids 48 us (4.4 TB/s), 64 x 131072 bf16 with 2048 ids 12.7 us.
+// 65537 float32: 97 us, 5.5 TB/s, rows at odd addresses); with one by the chain ids -> counters -> barrier -> stores, and every
+// chunk of a row looks at all of its ids: 256 x 100003 float32 with 4001 ids 45 us (4.6 TB/s), 64 x 131072 bf16 with 2048 ids
+// 12.9 us.  A row with a temperature or a penalty that has no normal reciprocal goes element by element; where that was a branch
+// in the unrolled loops, the others paid for it (64 x 131072: 12.3 against 11.7 us, fewer wavefronts a SIMD).
 template <class T, int THREADS, int VPT, class CNT, class B, bool BWD>
 __global__ __launch_bounds__(THREADS, 4) void k_logits_adjust(const AdjustArgs a, const AdjustGrid grid) {
   typedef typename T::comp comp;
@@ -393,7 +395,7 @@ template <class T, class B, bool BWD> __global__ __launch_bounds__(256) void k_l
 // Gradient of a bias that all rows share.  A workgroup of G groups of CT threads takes CT * kPer columns and a block of rows;
 // a thread owns kPer columns and every G-th row of the block, so that the column sums stay in its registers (float64) and
 // kSumRows rows are in flight; the groups are joined in LDS, the row blocks by k_logits_cols_final, all in a fixed order.
-// Without a history the gradient of the logits is written on the way.  4096 x 32768 bf16 with a mask: 130 us, 5.2 TB/s.
+// Without a history the gradient of the logits is written on the way.  4096 x 32768 bf16 with a mask: 123 us, 5.5 TB/s.
 constexpr int kSumThreads = 512, kSumRows = 4;
 
 template <class T, int CT, bool WRITE>
@@ -605,7 +607,7 @@ template <class T> M355_DEV void repack(raw_t<T>& r) {
 // again for the gradient.  The k % kPer last elements belong to the first threads, one each.  In place (grad == z): a row is
 // read before it is written, but for the pieces that are read again, which the same thread reads and writes.  Bound by HBM and
 // by how far the phases (load, sum, store) of the workgroups of a CU overlap: 4096 x 131072 bf16, an eighth of the rows padding,
-// 403 us (5.0 TB/s of what has to move, where a copy reaches 6.5), 1500 x 100003 float32 243 us.
+// 401 us (5.0 TB/s of what has to move, where a copy reaches 6.5), 1500 x 100003 float32 247 us.
 template <class T, int THREADS, int NR, int NL, int WAVES, bool REST>
 __global__ __launch_bounds__(THREADS, WAVES) void k_logits_grad(const DensityArgs a) {
   typedef typename T::comp comp;
@@ -816,7 +818,7 @@ template <class T, int G, bool GRAD> __global__ __launch_bounds__(256) void k_lo
 }
 
 // Value only: one row per workgroup, tiles of NR 16-byte loads per thread with a running maximum and sum.  Bound by HBM:
-// 8192 x 32768 float16 in 83 us, 6.5 TB/s.
+// 8192 x 32768 float16 in 85 us, 6.3 TB/s, a call among others (a launch that a profiler times by itself: 92-98 us).
 template <class T, int THREADS, int NR>
 __global__ __launch_bounds__(THREADS) void k_logits_value(const DensityArgs a) {
   constexpr int N = kPer<T>;
@@ -926,8 +928,9 @@ template <class T, int THREADS, int VPT, class CNT, class B, bool BWD> void laun
 
 template <class T, class B, bool BWD> void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   // Four pieces per thread hide the latencies of a chunk behind each other; where that gives too few workgroups for 256
-  // CUs, one piece each (1 x 32768 bf16, 300 ids: 4.4 against 5.4 us).  512 threads halve how often a history is scanned, and
-  // cost more than they save (512 x 131072 bf16, 500 ids: 77 against 71 us; 256 x 65536, 8000 ids: 41.0 against 42.3 us).
+  // CUs, one piece each (1 x 32768 bf16, 300 ids: 4.4 against 5.4 us).  512 threads halve how often a history is scanned:
+  // slower with a short one (512 x 131072 bf16, 500 ids: 77 against 71 us), 3 % faster with 8000 ids (256 x 65536: 41.0 against
+  // 42.3 us), which is not worth a second form.
   const bool few = a.rows * (a.k / kPer<T>) < 256ll * 1024;
   if (!a.history && a.k / kPer<T> < 256) {  // a workgroup per row would be half empty
     const int pieces = (int)((a.k + kPer<T> - 1) / kPer<T>);

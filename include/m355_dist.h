@@ -409,7 +409,8 @@ int m355_logits_logpdf(int64_t rows, int64_t k, int dtype, const void* logits, i
 /*
  * total = sum_r w_r logpdf_r (added in float64, in a fixed order) and, unless dlogits is NULL, its gradient
  *     dlogits[r, v] = w_r ((v == x_r) - exp(z_v) / sum exp(z))   (dtype; 0 where x_r is no category or the whole row is -inf)
- * weights: operand over the row index (float64 / float32 array or scalar).  A row of weight 0 contributes 0 and gets
+ * weights: operand over the row index (float64 / float32 array or scalar; the gradient takes them in the type of its
+ * arithmetic).  A row of weight 0 contributes 0 and gets
  * gradient 0, whatever it holds.  dlogits may be the logits themselves (same address and stride); any other overlap with
  * an input is undefined.  workspace: m355_logits_workspace_bytes bytes, 8-byte aligned, scratch; calls that may run
  * concurrently need one each.
